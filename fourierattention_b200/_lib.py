@@ -8,7 +8,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libfourier_b200.so")
 
-FA_DTYPE_F16, FA_DTYPE_BF16 = 0, 1
+FA_DTYPE_F16, FA_DTYPE_BF16, FA_DTYPE_F32 = 0, 1, 2
 FA_ANGLE_EXACT, FA_ANGLE_KM57 = 0, 1
 FA_DECODE_STATIC_SCRATCH_BYTES = 24 << 20
 
@@ -20,7 +20,8 @@ EXPORTS = ["fa_version", "fa_last_error_string", "fa_gather_cols", "fa_colstats"
            "fa_compress", "fa_evict_update", "fa_recon_stats_scratch_bytes", "fa_recon_stats", "fa_fourier_inverse",
            "fa_cache_step", "fa_evict_step", "fa_decode_scratch_bytes", "fa_decode_path", "fa_decode_attn", "fa_decode_attn_static", "fa_merge",
            "fa_layer_create", "fa_layer_destroy", "fa_layer_rebind_stores", "fa_layer_update", "fa_layer_scratch_bytes",
-           "fa_layer_attend", "fa_layer_decode_path"]
+           "fa_layer_attend", "fa_layer_decode_path", "fa_qk_norm_rope", "fa_paged_append", "fa_paged_attn_scratch_bytes",
+           "fa_paged_attn", "fa_sample"]
 
 i32, i64, vp, f32, sz = C.c_int32, C.c_int64, C.c_void_p, C.c_float, C.c_size_t
 
@@ -63,6 +64,37 @@ class LayerDesc(C.Structure):
         ("kc_list", vp), ("kc_h", vp), ("kn_list", vp), ("kn_h", vp),
         ("vc_list", vp), ("vc_h", vp), ("vn_list", vp), ("vn_h", vp),
         ("kn_h_host", vp), ("vn_h_host", vp),
+    ]
+
+
+class RopeArgs(C.Structure):
+    """Mirror of ``fa_rope_args_t``."""
+    _fields_ = [
+        ("tokens", i32), ("Hq", i32), ("Hkv", i32), ("D", i32), ("R", i32), ("dtype", i32), ("w_f32", i32),
+        ("pos_i64", i32),
+        ("q", vp), ("k", vp), ("v", vp),
+        ("q_st", i64), ("q_sh", i64), ("k_st", i64), ("k_sh", i64), ("v_st", i64), ("v_sh", i64),
+        ("q_out", vp), ("k_out", vp),
+        ("qo_st", i64), ("qo_sh", i64), ("ko_st", i64), ("ko_sh", i64),
+        ("positions", vp), ("inv_freq", vp), ("q_weight", vp), ("k_weight", vp), ("eps", f32),
+        ("B", i32), ("page_size", i32), ("max_pages", i32), ("num_pages", i32),
+        ("k_pages", vp), ("v_pages", vp),
+        ("kp_sp", i64), ("kp_sh", i64), ("kp_sr", i64), ("vp_sp", i64), ("vp_sh", i64), ("vp_sr", i64),
+        ("page_table", vp), ("table_sb", i64), ("kv_lens", vp), ("cu_seqlens", vp), ("pos_offset", i64),
+    ]
+
+
+class PagedAttnArgs(C.Structure):
+    """Mirror of ``fa_paged_attn_args_t``."""
+    _fields_ = [
+        ("tokens", i32), ("B", i32), ("Hq", i32), ("Hkv", i32), ("D", i32), ("page_size", i32), ("num_pages", i32),
+        ("max_pages", i32), ("n_prefix_pages", i32), ("prefix_len", i32), ("dtype", i32), ("sm_scale", f32),
+        ("q", vp), ("q_st", i64), ("q_sh", i64),
+        ("out", vp), ("o_st", i64), ("o_sh", i64), ("lse", vp),
+        ("k_pages", vp), ("v_pages", vp),
+        ("kp_sp", i64), ("kp_sh", i64), ("kp_sr", i64), ("vp_sp", i64), ("vp_sh", i64), ("vp_sr", i64),
+        ("page_table", vp), ("table_sb", i64), ("kv_lens", vp), ("cu_seqlens", vp), ("prefix_pages", vp),
+        ("scratch", vp), ("scratch_bytes", sz),
     ]
 
 
@@ -110,6 +142,12 @@ def _load():
     lib.fa_layer_scratch_bytes.restype = sz
     lib.fa_layer_attend.argtypes = [vp, i32, i32, i32, vp, i64, f32, vp, vp, vp, vp, sz, vp, vp]
     lib.fa_layer_decode_path.argtypes = [vp]
+    lib.fa_qk_norm_rope.argtypes = [C.POINTER(RopeArgs), vp]
+    lib.fa_paged_append.argtypes = [C.POINTER(RopeArgs), vp]
+    lib.fa_paged_attn_scratch_bytes.argtypes = [C.POINTER(PagedAttnArgs)]
+    lib.fa_paged_attn_scratch_bytes.restype = sz
+    lib.fa_paged_attn.argtypes = [C.POINTER(PagedAttnArgs), vp]
+    lib.fa_sample.argtypes = [vp, C.c_int, C.c_int, C.c_int, i64, vp, vp, f32, vp, C.c_int, vp, f32, vp, f32, vp, vp, vp]
     for name in EXPORTS:
         f = getattr(lib, name)
         if f.restype is C.c_int and name != "fa_version":

@@ -17,7 +17,8 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libfourier_b200.so")
-SOURCES = ["abi.cu", "cache_ops.cu", "compress.cu", "compress_tc.cu", "decode.cu"]
+SOURCES = ["abi.cu", "cache_ops.cu", "compress.cu", "compress_tc.cu", "decode.cu", "rope_append.cu", "paged_attn.cu",
+           "sample.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 

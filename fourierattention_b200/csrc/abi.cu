@@ -68,6 +68,23 @@ int make_tensor_map_3d(CUtensorMap* m, const void* base, int dtype, int cols, in
   return FA_OK;
 }
 
+int make_tensor_map_4d(CUtensorMap* m, const void* base, int dtype, int cols, int rows, int64_t row_stride, int heads,
+                       int64_t head_stride, int pages, int64_t page_stride, int box_cols, int box_rows) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  FA_REQUIRE(enc != nullptr, FA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)pages};
+  // the stride of a dimension of one entry is never used, but it has to be a valid one
+  cuuint64_t strides[3] = {(cuuint64_t)(rows > 1 ? row_stride : cols) * 2, (cuuint64_t)(heads > 1 ? head_stride : cols) * 2,
+                           (cuuint64_t)(pages > 1 ? page_stride : cols) * 2};
+  cuuint32_t box[4] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(m, dtype == FA_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                   const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  FA_REQUIRE(r == CUDA_SUCCESS, FA_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return FA_OK;
+}
+
 }  // namespace fa
 
 extern "C" int fa_version(void) { return 100; }

@@ -115,6 +115,10 @@ int sm_count();
 int make_tensor_map_3d(CUtensorMap* m, const void* base, int dtype, int cols, int rows, int64_t row_stride, int B,
                        int64_t batch_stride, int box_cols, int box_rows);
 
+// (cols x rows x heads x pages) tiled tensor map of a 16-bit cache of pages, 128-byte swizzle; the same limits.
+int make_tensor_map_4d(CUtensorMap* m, const void* base, int dtype, int cols, int rows, int64_t row_stride, int heads,
+                       int64_t head_stride, int pages, int64_t page_stride, int box_cols, int box_rows);
+
 // tensor-core projection (compress_tc.cu)
 bool compress_tc_usable(const void* x, int B, int K, int64_t x_sb, int64_t x_sk, int x_cols, int N);
 size_t compress_tc_scratch_bytes(int B, int K, int N, int x_cols);

@@ -1,0 +1,690 @@
+// Drawing one token per row of logits (fa_sample): temperature, top-k, top-p, min-p, and a given uniform number.
+//
+// With M the row's largest logit, w_i = exp((x_i - M) / temperature) and the order "larger logit first, lower index
+// first among equals", every filter keeps a head of that order:
+//   top-k: the first k;  top-p: the shortest head of those with sum >= p * (sum of the top-k head);  min-p: w_i >= min_p.
+// The token is the first index i (ascending) whose running sum of kept weights exceeds u * (their sum).
+//
+// Nothing is sorted as a whole.  A head of the order is {x > t} plus the ties at t up to an index, so each of top-k and
+// top-p is a search for one element: a histogram of M - x over 1024 equal bins finds the bin it is in, the bin's
+// elements (up to LIST of them) are ranked against one another, and a fuller bin is split again, down to bins of one
+// value whose ties are counted in the order of their indices.  Whether a token is in hangs on sums next to a border,
+// and one token too many or too few changes the draw, so every sum that decides is taken in float64 in a fixed order;
+// the histogram of top-p (integers: the same whatever the order of the atomics) only proposes a bin, which the
+// float64 sums then confirm or move.
+//
+// Layout: a cluster of 1 to 8 CTAs holds a row in shared memory (float32, read from HBM once; a thread owns up
+// to 32 neighbouring elements, one word of padding per 32 keeps its walk free of bank conflicts) and exchanges partial
+// results through distributed shared memory: every CTA reads all of them and decides alike, one cluster barrier per
+// step.  Bound: latency of those steps for few rows, issue of the float64 exponentials for many.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace fa {
+
+constexpr int SA_THREADS = 512;
+constexpr int SA_WARPS = SA_THREADS / 32;
+constexpr int SA_EPT = 32;                         // most neighbouring elements of a thread, per round
+constexpr int SA_ROUND = SA_THREADS * SA_EPT;      // elements of a CTA, per round
+constexpr int SA_MAX_ROUNDS = 3;
+constexpr int SA_MAX_CLUSTER = 8;
+constexpr int SA_BINS = 1024;
+constexpr int SA_LIST = 512;
+constexpr int SA_MAX_VOCAB = SA_MAX_CLUSTER * SA_MAX_ROUNDS * SA_ROUND;
+
+struct SampleParams {
+  const void* logits;
+  int64_t sb;
+  int V, slice, ept, rounds;      // elements of a CTA, of a thread per round; rounds of SA_ROUND elements
+  const float *u, *temperature, *top_p, *min_p;    // per row, or null: the value below
+  const int32_t* top_k;
+  float temperature0, top_p0, min_p0;
+  int top_k0;
+  int64_t* token;
+  float* logprob;
+};
+
+struct SaXchg {
+  double s[2];
+  float f[2];
+  int n[2];
+};
+
+struct SaShared {
+  uint32_t hist[SA_BINS];
+  SaXchg x[2];
+  float lx[SA_LIST];          // this CTA's part of a bin
+  int li[SA_LIST];
+  unsigned ln;
+  float gx[SA_LIST];          // the bin of the whole cluster
+  int gi[SA_LIST];
+  double gw[SA_LIST];         // its weights, in order
+  float ox[SA_LIST];
+  int oi[SA_LIST];
+  double red_d[2][SA_WARPS];
+  float red_f[2][SA_WARPS];
+  int red_n[2][SA_WARPS];
+  int pick;
+  double pick_d;
+  int pick_i;
+};
+
+__device__ __forceinline__ double shfl_up_d(double v, int o) { return __shfl_up_sync(0xffffffffu, v, o); }
+__device__ __forceinline__ double warp_sum_d(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ float sa_value(T v) {
+  const float f = to_f32(v);
+  return f != f ? -INFINITY : f;       // NaN: never drawn
+}
+template <>
+__device__ __forceinline__ float sa_value<float>(float f) {
+  return f != f ? -INFINITY : f;
+}
+
+template <typename T>
+struct Sampler {
+  const SampleParams& p;
+  SaShared& sh;
+  float* xs;
+  cg::cluster_group cl;
+  int rank, size, n, base, xb;         // CTA of the cluster; elements held, index of the first
+  int tid, lane, warp;
+  float M;
+  double inv_t;
+  // the head kept so far: x > kx, or x == kx and index <= ki
+  float kx;
+  int ki;
+
+  __device__ __forceinline__ float& at(int i) { return xs[i + (i >> 5)]; }
+  __device__ __forceinline__ double weight(float x) const { return exp((double)(x - M) * inv_t); }
+  __device__ __forceinline__ bool kept(float x, int i) const { return x > kx || (x == kx && i <= ki); }
+
+  template <typename F>
+  __device__ __forceinline__ void each(F f) {
+    for (int r = 0; r < p.rounds; ++r) {
+      const int i0 = r * SA_ROUND + tid * p.ept, i1 = min(n, i0 + p.ept);
+      for (int i = i0; i < i1; ++i) f(at(i), base + i);
+    }
+  }
+
+  // sums over the cluster, in a fixed order: lanes, warps, CTAs.  Every CTA returns the same.
+  __device__ __forceinline__ void exchange(double s0, double s1, float mn, float mx, int n0, int n1, SaXchg& out) {
+    s0 = warp_sum_d(s0), s1 = warp_sum_d(s1);
+    mn = -warp_max(-mn), mx = warp_max(mx);
+    n0 = __reduce_add_sync(0xffffffffu, n0), n1 = __reduce_add_sync(0xffffffffu, n1);
+    __syncthreads();
+    if (lane == 0) {
+      sh.red_d[0][warp] = s0, sh.red_d[1][warp] = s1;
+      sh.red_f[0][warp] = mn, sh.red_f[1][warp] = mx;
+      sh.red_n[0][warp] = n0, sh.red_n[1][warp] = n1;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      SaXchg o = {{0.0, 0.0}, {INFINITY, -INFINITY}, {0, 0}};
+      for (int w = 0; w < SA_WARPS; ++w) {
+        o.s[0] += sh.red_d[0][w], o.s[1] += sh.red_d[1][w];
+        o.f[0] = fminf(o.f[0], sh.red_f[0][w]), o.f[1] = fmaxf(o.f[1], sh.red_f[1][w]);
+        o.n[0] += sh.red_n[0][w], o.n[1] += sh.red_n[1][w];
+      }
+      sh.x[xb] = o;
+    }
+    cl.sync();
+    out = {{0.0, 0.0}, {INFINITY, -INFINITY}, {0, 0}};
+    for (int r = 0; r < size; ++r) {
+      const SaXchg o = *cl.map_shared_rank(&sh.x[xb], r);
+      out.s[0] += o.s[0], out.s[1] += o.s[1];
+      out.f[0] = fminf(out.f[0], o.f[0]), out.f[1] = fmaxf(out.f[1], o.f[1]);
+      out.n[0] += o.n[0], out.n[1] += o.n[1];
+    }
+    xb ^= 1;
+  }
+
+  // index of the m-th (from 0) element equal to x in the order of the indices
+  __device__ int nth_tie(float x, int m) {
+    int mine = 0;
+    each([&](float v, int i) { mine += kept(v, i) && v == x; });
+    if (p.rounds == 1) {
+      // counts by thread are in the order of the indices
+      int inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      return tie_locate(x, m, inc - mine, mine, 0, __shfl_sync(0xffffffffu, inc, 31));
+    }
+    return tie_rounds(x, m);
+  }
+  __device__ int tie_locate(float x, int m, int excl, int mine, int round, int wtotal) {
+    __syncthreads();
+    if (lane == 31) sh.red_n[0][warp] = wtotal;
+    if (tid == 0) sh.pick_i = -1;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < SA_WARPS; ++w) {
+      if (w < warp) before += sh.red_n[0][w];
+      all += sh.red_n[0][w];
+    }
+    if (tid == 0) sh.x[xb].n[0] = all;
+    cl.sync();
+    int pre = 0;
+    for (int r = 0; r < rank; ++r) pre += cl.map_shared_rank(&sh.x[xb], r)->n[0];
+    int k = m - pre - before - excl;
+    if (k >= 0 && k < mine) {
+      const int i0 = round * SA_ROUND + tid * p.ept, i1 = min(n, i0 + p.ept);
+      for (int i = i0; i < i1; ++i)
+        if (kept(at(i), base + i) && at(i) == x && k-- == 0) sh.pick_i = base + i;
+    }
+    xb ^= 1;
+    __syncthreads();
+    return share_pick();
+  }
+  // the index found by one thread of the cluster, to all
+  __device__ int share_pick() {
+    if (tid == 0) sh.x[xb].n[0] = sh.pick_i;
+    cl.sync();
+    int found = -1;
+    for (int r = 0; r < size; ++r) found = max(found, cl.map_shared_rank(&sh.x[xb], r)->n[0]);
+    xb ^= 1;
+    return found;
+  }
+  // several rounds: CTAs hold whole ranges of indices, so the CTA first, then its rounds one by one
+  __device__ int tie_rounds(float x, int m) {
+    int mine = 0;
+    each([&](float v, int i) { mine += kept(v, i) && v == x; });
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    __syncthreads();
+    if (lane == 0) sh.red_n[0][warp] = mine;
+    if (tid == 0) sh.pick_i = -1;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < SA_WARPS; ++w) all += sh.red_n[0][w];
+    if (tid == 0) sh.x[xb].n[0] = all;
+    cl.sync();
+    int k = m;
+    for (int r = 0; r < rank; ++r) k -= cl.map_shared_rank(&sh.x[xb], r)->n[0];
+    xb ^= 1;
+    if (k >= 0 && k < all) {
+      for (int r = 0; r < p.rounds; ++r) {
+        const int i0 = r * SA_ROUND + tid * p.ept, i1 = min(n, i0 + p.ept);
+        int c = 0;
+        for (int i = i0; i < i1; ++i) c += kept(at(i), base + i) && at(i) == x;
+        int inc = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += v;
+        }
+        __syncthreads();
+        if (lane == 31) sh.red_n[0][warp] = inc;
+        __syncthreads();
+        int before = 0, tot = 0;
+        for (int w = 0; w < SA_WARPS; ++w) {
+          if (w < warp) before += sh.red_n[0][w];
+          tot += sh.red_n[0][w];
+        }
+        int j = k - before - (inc - c);
+        if (j >= 0 && j < c)
+          for (int i = i0; i < i1; ++i)
+            if (kept(at(i), base + i) && at(i) == x && j-- == 0) sh.pick_i = base + i;
+        k -= tot;
+      }
+    }
+    __syncthreads();
+    return share_pick();
+  }
+
+  // Shortens the kept head: to its first `k` elements (by_weight false), or to the shortest one whose weight reaches
+  // `goal` (by_weight true; `part` is the weight of the whole kept head).  Its logits are in [lo, hi].
+  __device__ void shorten(bool by_weight, int k, double goal, double part, float lo, float hi) {
+    double near = 0.0;                 // what lies above hi: a number of elements or a weight
+    for (int level = 0; level < 256; ++level) {
+      // a bin number that never falls with hi - x, whatever the rounding; 0 for hi and the last one for lo, so that
+      // every level separates the two
+      const float half = hi - lo < INFINITY ? 1.f : 0.5f;
+      const float top = half * hi, range = top - half * lo, scale = (float)SA_BINS / range;
+      auto bin_of = [&](float x) { return min(SA_BINS - 1, (int)(fmaf(-half, x, top) * scale)); };
+      const float width = range / (float)SA_BINS / half, c_w = (float)inv_t;
+      __syncthreads();
+      for (int i = tid; i < SA_BINS; i += SA_THREADS) sh.hist[i] = 0;
+      __syncthreads();
+      each([&](float x, int i) {
+        if (!kept(x, i) || x > hi || x < lo) return;
+        const int b = bin_of(x);
+        // weights relative to the bin's near edge, in steps of 2^-14: a CTA's part of a bin stays below 2^30
+        const float rel = fminf(0.f, (x - hi + (float)b * width) * c_w);
+        atomicAdd(&sh.hist[b], by_weight ? max(1u, __float2uint_rn(16384.f * __expf(rel))) : 1u);
+      });
+      cl.sync();
+      // two neighbouring bins per thread, over the cluster
+      double v0 = 0.0, v1 = 0.0;
+      for (int r = 0; r < size; ++r) {
+        const uint2 h = *reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh.hist[2 * tid], r));
+        v0 += (double)h.x, v1 += (double)h.y;
+      }
+      if (by_weight) {
+        // relative to the weight at hi
+        v0 *= exp((double)(2 * tid * width) * -inv_t);
+        v1 *= exp((double)((2 * tid + 1) * width) * -inv_t);
+      }
+      double pre = v0 + v1;              // running sum up to and with this thread's bins
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double v = shfl_up_d(pre, o);
+        if (lane >= o) pre += v;
+      }
+      __syncthreads();
+      if (lane == 31) sh.red_d[0][warp] = pre;
+      __syncthreads();
+      double total = 0.0;
+      for (int w = 0; w < SA_WARPS; ++w) {
+        if (w < warp) pre += sh.red_d[0][w];
+        total += sh.red_d[0][w];
+      }
+      pre -= v0 + v1;
+      // the histogram's weights are in units of their own, `unit` of them make one of the exact sums
+      const double unit = by_weight ? total / part : 1.0;
+      double target = by_weight ? fmin((goal - near) * unit, total) : (double)k - near;
+
+      // ---- the bin's elements, and what lies before it --------------------------------------------------------
+      int b_min = 0, b_max = SA_BINS - 1;
+      bool split = false;
+      while (b_min <= b_max) {
+        __syncthreads();
+        if (tid == 0) sh.pick = b_max, sh.ln = 0;
+        __syncthreads();
+        if (v0 > 0.0 && pre + v0 >= target) atomicMin(&sh.pick, 2 * tid);
+        else if (v1 > 0.0 && pre + v0 + v1 >= target) atomicMin(&sh.pick, 2 * tid + 1);
+        __syncthreads();
+        const int b = max(sh.pick, b_min);
+        if (2 * tid == (b & ~1)) sh.pick_d = (b & 1) ? pre + v0 : pre;
+        double s_before = 0.0, s_in = 0.0;
+        float mn = INFINITY, mx = -INFINITY;
+        int n_in = 0, n_before = 0;
+        each([&](float x, int i) {
+          if (!kept(x, i) || x < lo) return;
+          const int bb = x > hi ? -1 : bin_of(x);
+          if (bb > b) return;
+          const double w = by_weight ? weight(x) : 0.0;
+          if (bb < b) {
+            s_before += w;
+            ++n_before;
+          } else {
+            s_in += w;
+            ++n_in;
+            mn = fminf(mn, x), mx = fmaxf(mx, x);
+            const unsigned slot = atomicAdd(&sh.ln, 1u);
+            if (slot < SA_LIST) sh.lx[slot] = x, sh.li[slot] = i;
+          }
+        });
+        SaXchg o;
+        exchange(s_before, s_in, mn, mx, n_before, n_in, o);
+        if (by_weight) {
+          // the answer is in this bin if the exact sum passes the goal inside it; else the proposal is made again from
+          // the sum as it is, among the bins not ruled out
+          const int move = o.s[0] >= goal && o.n[0] > 0 ? -1 : o.s[0] + o.s[1] < goal ? 1 : 0;
+          if (move < 0) b_max = b - 1;
+          if (move > 0) b_min = b + 1;
+          if (move != 0 && b_min <= b_max) {
+            target = (goal - o.s[0]) * unit + sh.pick_d;
+            cl.sync();                        // the lists are written anew
+            continue;
+          }
+        }
+        if (o.n[1] == 0) return;              // nothing to cut
+        if (o.f[0] == o.f[1]) {
+          cut_ties(o.f[0], by_weight, k, goal, o);
+          return;
+        }
+        if (o.n[1] <= SA_LIST) {
+          rank_list(o.n[1], by_weight, k - o.n[0], o.s[0], goal);
+          return;
+        }
+        lo = o.f[0], hi = o.f[1];
+        near = by_weight ? o.s[0] : (double)o.n[0];
+        part = o.s[1];
+        split = true;
+        break;
+      }
+      if (!split) return;
+      cl.sync();
+    }
+  }
+
+  // the bin is one value: its first m ties are kept
+  __device__ void cut_ties(float x, bool by_weight, int k, double goal, const SaXchg& o) {
+    int m = k - o.n[0];
+    if (by_weight) {
+      const double w = weight(x);
+      m = (int)fmin((double)o.n[1], fmax(1.0, ceil((goal - o.s[0]) / w)));
+      while (m > 1 && o.s[0] + (double)(m - 1) * w >= goal) --m;
+      while (m < o.n[1] && o.s[0] + (double)m * w < goal) ++m;
+    }
+    m = max(1, min(m, o.n[1]));
+    const int last = m == o.n[1] ? 0x7fffffff : nth_tie(x, m - 1);
+    ki = x == kx ? min(ki, last) : last;
+    kx = x;
+  }
+
+  // orders the n listed elements of the cluster and cuts the kept head at one of them
+  __device__ void rank_list(int n_all, bool by_weight, int k, double before, double goal) {
+    int off = 0;
+    for (int r = 0; r < size; ++r) {
+      const int c = (int)*cl.map_shared_rank(&sh.ln, r);
+      for (int i = tid; i < c; i += SA_THREADS) {
+        sh.gx[off + i] = *cl.map_shared_rank(&sh.lx[i], r);
+        sh.gi[off + i] = *cl.map_shared_rank(&sh.li[i], r);
+      }
+      off += c;
+    }
+    __syncthreads();
+    for (int e = tid; e < n_all; e += SA_THREADS) {
+      const float x = sh.gx[e];
+      const int i = sh.gi[e];
+      int rk = 0;
+      for (int j = 0; j < n_all; ++j) rk += sh.gx[j] > x || (sh.gx[j] == x && sh.gi[j] < i);
+      sh.ox[rk] = x, sh.oi[rk] = i;
+      sh.gw[rk] = by_weight ? weight(x) : 0.0;
+    }
+    if (tid == 0) sh.pick = n_all - 1;
+    __syncthreads();
+    if (by_weight) {
+      // running sum over at most SA_THREADS elements, one per thread
+      double inc = tid < n_all ? sh.gw[tid] : 0.0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double v = shfl_up_d(inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (lane == 31) sh.red_d[0][warp] = inc;
+      __syncthreads();
+      double pre = before;
+      for (int w = 0; w < warp; ++w) pre += sh.red_d[0][w];
+      if (tid < n_all && pre + inc >= goal) atomicMin(&sh.pick, tid);
+      __syncthreads();
+    } else if (tid == 0) {
+      sh.pick = max(0, min(k - 1, n_all - 1));
+    }
+    __syncthreads();
+    kx = sh.ox[sh.pick];
+    ki = sh.oi[sh.pick];
+    __syncthreads();
+  }
+
+  __device__ void run(int row) {
+    const T* x = reinterpret_cast<const T*>(p.logits) + (int64_t)row * p.sb;
+    xb = 0;
+    base = rank * p.slice;
+    n = max(0, min(p.V - base, p.slice));
+    const float temperature = p.temperature ? p.temperature[row] : p.temperature0;
+    const float top_p = p.top_p ? p.top_p[row] : p.top_p0;
+    const float min_p = p.min_p ? p.min_p[row] : p.min_p0;
+    int top_k = p.top_k ? p.top_k[row] : p.top_k0;
+    // ---- the row, once ------------------------------------------------------------------------------------------
+    float mn = INFINITY, mx = -INFINITY;
+    int fin = 0;
+    auto take = [&](int i, float v) {
+      at(i) = v;
+      mx = fmaxf(mx, v);
+      if (v > -INFINITY) {
+        ++fin;
+        mn = fminf(mn, v);
+      }
+    };
+    // 16-byte loads behind the first aligned element, single ones before and after
+    constexpr int VL = 16 / (int)sizeof(T);
+    const T* src = x + base;
+    const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(T)));
+    const int nv = (n - head) / VL;
+    if (tid < head) take(tid, sa_value<T>(src[tid]));
+    for (int i = head + nv * VL + tid; i < n; i += SA_THREADS) take(i, sa_value<T>(src[i]));
+    const uint4* vec = reinterpret_cast<const uint4*>(src + head);
+    constexpr int U = 4;               // loads in flight per thread
+    for (int v0 = tid; v0 < nv; v0 += U * SA_THREADS) {
+      uint4 raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (v0 + u * SA_THREADS < nv) raw[u] = __ldg(vec + v0 + u * SA_THREADS);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (v0 + u * SA_THREADS >= nv) break;
+        const T* e = reinterpret_cast<const T*>(&raw[u]);
+#pragma unroll
+        for (int j = 0; j < VL; ++j) take(head + (v0 + u * SA_THREADS) * VL + j, sa_value<T>(e[j]));
+      }
+    }
+    SaXchg o;
+    exchange(0.0, 0.0, mn, mx, fin, 0, o);
+    M = o.f[1];
+    int n_fin = o.n[0];
+    float low = o.f[0];
+    kx = -INFINITY, ki = -1;               // everything above -infinity
+    if (n_fin == 0) {
+      // no logit to draw from
+      if (rank == 0 && tid == 0) {
+        p.token[row] = -1;
+        if (p.logprob) p.logprob[row] = -INFINITY;
+      }
+      return;
+    }
+    if (M == INFINITY) {
+      // the limit of ever larger logits: those at +infinity share the probability
+      int c = 0;
+      for (int i = tid; i < n; i += SA_THREADS) {
+        at(i) = at(i) == INFINITY ? 0.f : -INFINITY;
+        c += at(i) == 0.f;
+      }
+      exchange(0.0, 0.0, 0.f, 0.f, c, 0, o);
+      M = 0.f, low = 0.f, n_fin = o.n[0];
+    }
+    inv_t = temperature > 0.f ? 1.0 / (double)temperature : 0.0;
+    if (!(temperature > 0.f)) top_k = 1;   // the largest logit, lowest index
+    if (top_k > 0 && top_k < n_fin) shorten(false, top_k, 0.0, 0.0, low, M);
+    if (top_p < 1.f && top_k != 1) {
+      double s = 0.0;
+      each([&](float v, int i) {
+        if (kept(v, i)) s += weight(v);
+      });
+      exchange(s, 0.0, 0.f, 0.f, 0, 0, o);
+      shorten(true, 0, (double)fmaxf(top_p, 0.f) * o.s[0], o.s[0], kx > -INFINITY ? kx : low, M);
+    }
+    draw(row, (double)p.u[row], (double)min_p);
+  }
+
+  __device__ void draw(int row, double u, double min_p) {
+    double W = 0.0;
+    auto mass = [&](int i) -> double {
+      const float v = at(i);
+      if (!kept(v, base + i)) return 0.0;
+      const double w = weight(v);
+      return w >= min_p || v == M ? w : 0.0;
+    };
+    double mine[SA_MAX_ROUNDS], s = 0.0;
+#pragma unroll
+    for (int r = 0; r < SA_MAX_ROUNDS; ++r) {
+      mine[r] = 0.0;
+      if (r >= p.rounds) continue;
+      const int i0 = r * SA_ROUND + tid * p.ept, i1 = min(n, i0 + p.ept);
+      for (int i = i0; i < i1; ++i) mine[r] += mass(i);
+      s += mine[r];
+    }
+    // the CTA's sum, and those of the CTAs before it
+    s = warp_sum_d(s);
+    __syncthreads();
+    if (lane == 0) sh.red_d[0][warp] = s;
+    if (tid == 0) sh.pick_i = -1;
+    __syncthreads();
+    if (tid == 0) {
+      double t = 0.0;
+      for (int w = 0; w < SA_WARPS; ++w) t += sh.red_d[0][w];
+      sh.x[xb].s[0] = t;
+    }
+    cl.sync();
+    double pre = 0.0;
+    int owner = 0;
+    double own_pre = 0.0;
+    for (int r = 0; r < size; ++r) W += cl.map_shared_rank(&sh.x[xb], r)->s[0];
+    const double goal = u * W;
+    for (int r = 0; r < size; ++r) {
+      const double c = cl.map_shared_rank(&sh.x[xb], r)->s[0];
+      if (c > 0.0) owner = r, own_pre = pre;         // the last CTA with weight, unless one before it passes the goal
+      if (pre + c > goal) break;
+      pre += c;
+    }
+    xb ^= 1;
+    if (rank == owner) {
+      double before = own_pre;
+#pragma unroll
+      for (int r = 0; r < SA_MAX_ROUNDS; ++r) {
+        if (r >= p.rounds) break;
+        double inc = mine[r];
+#pragma unroll
+        for (int of = 1; of < 32; of <<= 1) {
+          const double v = shfl_up_d(inc, of);
+          if (lane >= of) inc += v;
+        }
+        __syncthreads();
+        if (lane == 31) sh.red_d[1][warp] = inc;
+        __syncthreads();
+        double at0 = before;
+        for (int w = 0; w < warp; ++w) at0 += sh.red_d[1][w];
+        const double hi_s = at0 + inc;
+        // the first thread whose sum passes the goal; the last one with weight as a fallback for u -> 1
+        if (mine[r] > 0.0) {
+          const int key = r * SA_THREADS + tid;
+          if (hi_s > goal) atomicMin(reinterpret_cast<unsigned*>(&sh.pick_i), (unsigned)key);
+        }
+        for (int w = warp; w < SA_WARPS; ++w) at0 += sh.red_d[1][w];
+        before = at0;
+      }
+      __syncthreads();
+      finish(row, goal, own_pre, W, mine, mass);
+    }
+  }
+
+  template <typename F>
+  __device__ void finish(int row, double goal, double own_pre, double W, const double* mine, F mass) {
+    unsigned key = (unsigned)sh.pick_i;
+    if (key == 0xffffffffu) {
+      // rounding at the very end: the last thread with weight
+      __syncthreads();
+      int last = -1;
+#pragma unroll
+      for (int r = 0; r < SA_MAX_ROUNDS; ++r)
+        if (mine[r] > 0.0) last = r * SA_THREADS + tid;
+      last = __reduce_max_sync(0xffffffffu, last);
+      if (lane == 0) sh.red_n[1][warp] = last;
+      __syncthreads();
+      for (int w = 0; w < SA_WARPS; ++w) last = max(last, sh.red_n[1][w]);
+      key = (unsigned)last;
+    }
+    // the sum before that thread, in the order of the indices
+    const int kr = key / SA_THREADS, kt = key % SA_THREADS;
+    double before = own_pre;
+#pragma unroll
+    for (int r = 0; r < SA_MAX_ROUNDS; ++r) {
+      if (r > kr) break;
+      double v = (r < kr || tid < kt) ? mine[r] : 0.0;
+      v = warp_sum_d(v);
+      __syncthreads();
+      if (lane == 0) sh.red_d[0][warp] = v;
+      __syncthreads();
+      for (int w = 0; w < SA_WARPS; ++w) before += sh.red_d[0][w];
+    }
+    if (tid == 0) {
+      const int i0 = kr * SA_ROUND + kt * p.ept, i1 = min(n, i0 + p.ept);
+      double run_sum = before, wt = 0.0;
+      int token = -1;
+      for (int i = i0; i < i1; ++i) {
+        const double w = mass(i);
+        if (w > 0.0) token = base + i, wt = w;
+        run_sum += w;
+        if (w > 0.0 && run_sum > goal) break;
+      }
+      p.token[row] = token;
+      if (p.logprob) p.logprob[row] = (float)log(wt / W);
+    }
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(SA_THREADS) sample_kernel(const SampleParams p) {
+  extern __shared__ float sa_xs[];
+  __shared__ SaShared sh;
+  cg::cluster_group cl = cg::this_cluster();
+  Sampler<T> s{p, sh, sa_xs, cl};
+  s.rank = (int)cl.block_rank(), s.size = (int)cl.num_blocks();
+  s.tid = threadIdx.x, s.lane = threadIdx.x & 31, s.warp = threadIdx.x >> 5;
+  s.run(blockIdx.x / s.size);
+  cl.sync();       // no CTA leaves while another may still read its shared memory
+}
+
+template <typename T>
+static int sample_launch(const SampleParams& prm, int B, int cluster, cudaStream_t st) {
+  const int smem = prm.rounds * SA_THREADS * (SA_EPT + 1) * 4;
+  cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       SA_MAX_ROUNDS * SA_THREADS * (SA_EPT + 1) * 4);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(sample)");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(B * cluster);
+  cfg.blockDim = dim3(SA_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, prm);
+  if (e != cudaSuccess) return cuda_fail(e, "fa_sample");
+  return FA_OK;
+}
+
+}  // namespace fa
+
+using namespace fa;
+
+extern "C" int fa_sample(const void* logits, int dtype, int B, int V, int64_t logits_sb, const float* u,
+                         const float* temperature, float temperature0, const int32_t* top_k, int top_k0,
+                         const float* top_p, float top_p0, const float* min_p, float min_p0, int64_t* token,
+                         float* logprob, fa_stream_t stream) {
+  FA_REQUIRE(dtype == FA_DTYPE_F16 || dtype == FA_DTYPE_BF16 || dtype == FA_DTYPE_F32, FA_ERR_DTYPE,
+             "fa_sample: bad dtype %d", dtype);
+  FA_REQUIRE(B >= 0 && V > 0, FA_ERR_SHAPE, "fa_sample: bad sizes (%d rows of %d logits)", B, V);
+  FA_REQUIRE(V <= SA_MAX_VOCAB, FA_ERR_CAPACITY, "fa_sample: %d logits in a row, at most %d are held", V, SA_MAX_VOCAB);
+  if (B == 0) return FA_OK;
+  FA_REQUIRE(logits && u && token, FA_ERR_NULL, "fa_sample: null pointer");
+  // A row takes as many CTAs as it has rounds of 16384 elements to keep one round each; with rows enough for only a
+  // part of the GPU it is spread further, down to 2048 elements per CTA.
+  int cluster = 1;
+  while (cluster < SA_MAX_CLUSTER && (ceil_div(V, cluster) > SA_ROUND ||
+                                      ((int64_t)B * cluster * 2 <= sm_count() && ceil_div(V, 2 * cluster) >= 2048)))
+    cluster *= 2;
+  SampleParams prm;
+  prm.logits = logits;
+  prm.sb = logits_sb;
+  prm.V = V;
+  prm.slice = ceil_div(V, cluster);
+  prm.rounds = ceil_div(prm.slice, SA_ROUND);
+  prm.ept = prm.rounds > 1 ? SA_EPT : ceil_div(prm.slice, SA_THREADS);
+  prm.u = u;
+  prm.temperature = temperature, prm.temperature0 = temperature0;
+  prm.top_k = top_k, prm.top_k0 = top_k0;
+  prm.top_p = top_p, prm.top_p0 = top_p0;
+  prm.min_p = min_p, prm.min_p0 = min_p0;
+  prm.token = token;
+  prm.logprob = logprob;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == FA_DTYPE_F32) return sample_launch<float>(prm, B, cluster, st);
+  if (dtype == FA_DTYPE_F16) return sample_launch<__half>(prm, B, cluster, st);
+  return sample_launch<__nv_bfloat16>(prm, B, cluster, st);
+}

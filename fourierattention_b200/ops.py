@@ -457,6 +457,263 @@ def merge(o, m, l):
     return out
 
 
+# ---- a served batch outside the compressed span: norm + rotation, paged cache, shared prefix, sampling ------------------
+
+def _on(dev, *ts):
+    """Every given tensor on ``dev``, a CUDA device."""
+    if dev.type != "cuda":
+        raise RuntimeError("fourierattention_b200 kernels need CUDA tensors (there is no CPU path)")
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on different devices: {t.device} and {dev}")
+
+
+def _no_grad(*ts):
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("this operator has no backward pass: call it under torch.no_grad()")
+
+
+def _heads3(t, name, dtype=None):
+    """Sizes of a (tokens, heads, D) tensor with a contiguous last dimension."""
+    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+        raise ValueError(f"{name}: expected (tokens, heads, head_dim) with a contiguous last dimension")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name}: expected dtype {dtype}, got {t.dtype}")
+    return t.shape
+
+
+def _int32(t, name, shape):
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or (t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise ValueError(f"{name}: expected int32 {shape} with a contiguous last dimension, "
+                         f"got {t.dtype} {tuple(t.shape)}")
+
+
+def _call(fn, name, dev, *args):
+    """One call of the library on the current stream of ``dev``."""
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if rc:
+        check(rc, name)
+
+
+def _rope_args(a, q, k, inv_freq, q_weight, k_weight, eps, q_out):
+    """The part of the argument block that qk_norm_rope and paged_append share; returns the query output."""
+    ref = q if q is not None else k
+    a.dtype = _dt(ref)
+    tokens, heads, D = _heads3(ref, "q" if q is not None else "k")
+    a.tokens, a.D = tokens, D
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq: expected a contiguous float32 vector")
+    a.R, a.inv_freq = 2 * inv_freq.shape[0], inv_freq.data_ptr()
+    if k is not None:
+        if k is not ref and _heads3(k, "k", ref.dtype)[::2] != (tokens, D):
+            raise ValueError("q and k must have the same tokens and head dimension")
+        a.Hkv, a.k, a.k_st, a.k_sh = k.shape[1], k.data_ptr(), k.stride(0), k.stride(1)
+    if q is not None:
+        if q_out is None:
+            q_out = torch.empty((tokens, heads, D), dtype=q.dtype, device=q.device)
+        elif _heads3(q_out, "q_out", q.dtype) != q.shape:
+            raise ValueError("q_out must have the shape of q")
+        a.Hq, a.q, a.q_st, a.q_sh = heads, q.data_ptr(), q.stride(0), q.stride(1)
+        a.q_out, a.qo_st, a.qo_sh = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is None:
+            continue
+        if tuple(w.shape) != (D,) or not w.is_contiguous() or w.dtype not in (ref.dtype, torch.float32):
+            raise ValueError(f"{name}: expected a contiguous ({D},) tensor of {ref.dtype} or float32")
+        if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+            raise ValueError("q_weight and k_weight must share their dtype")
+        a.w_f32 = 1 if w.dtype == torch.float32 else 0
+        setattr(a, name, w.data_ptr())
+    a.eps = eps
+    return q_out
+
+
+def _positions(a, positions, tokens):
+    if positions.dtype not in (torch.int64, torch.int32) or tuple(positions.shape) != (tokens,) \
+            or not positions.is_contiguous():
+        raise ValueError(f"positions: expected a contiguous int64 or int32 ({tokens},) tensor")
+    a.positions, a.pos_i64 = positions.data_ptr(), 1 if positions.dtype == torch.int64 else 0
+
+
+def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, q_out=None, k_out=None):
+    """RMS norm of every query and key head (where a weight is given) and the rotation by position, in one pass.
+    q: (tokens, Hq, D), k: (tokens, Hkv, D), any strides with a contiguous last dimension (views of a fused projection);
+    positions: (tokens,) int64 or int32; inv_freq: (R/2,) float32, R <= D a multiple of 16 (rotated pairs are
+    ``(i, i + R/2)``, dims from R on are passed through); weights: (D,) of the model dtype or float32.  float32
+    arithmetic with exact angles, one rounding.  Returns (q, k), written to ``q_out`` / ``k_out`` if given (the inputs
+    themselves are allowed)."""
+    _no_grad(q, k, q_weight, k_weight)
+    a = _lib.RopeArgs()
+    _heads3(q, "q")
+    q_out = _rope_args(a, q, k, inv_freq, q_weight, k_weight, eps, q_out)
+    _positions(a, positions, q.shape[0])
+    if k_out is None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    elif _heads3(k_out, "k_out", k.dtype) != k.shape:
+        raise ValueError("k_out must have the shape of k")
+    a.k_out, a.ko_st, a.ko_sh = k_out.data_ptr(), k_out.stride(0), k_out.stride(1)
+    _on(q.device, k, positions, inv_freq, q_weight, k_weight, q_out, k_out)
+    _call(lib.fa_qk_norm_rope, "fa_qk_norm_rope", q.device, C.byref(a))
+    _count(1)
+    return q_out, k_out
+
+
+def _pages(a, k_pages, v_pages, dtype, Hkv, D):
+    """Sizes and strides of a cache of pages (num_pages, Hkv, page_size, D)."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != dtype or v_pages.dtype != dtype \
+            or k_pages.shape[1] != Hkv or k_pages.shape[3] != D or k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+        raise ValueError(f"k_pages, v_pages: expected {dtype} (num_pages, {Hkv}, page_size, {D}) with a contiguous last "
+                         "dimension")
+    a.num_pages, a.page_size = k_pages.shape[0], k_pages.shape[2]
+    a.k_pages, a.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
+    a.kp_sp, a.kp_sh, a.kp_sr, _ = k_pages.stride()
+    a.vp_sp, a.vp_sh, a.vp_sr, _ = v_pages.stride()
+
+
+def _sequences(a, page_table, kv_lens, cu_seqlens, tokens):
+    if page_table.dim() != 2:
+        raise ValueError("page_table: expected int32 (sequences, pages)")
+    B, most = page_table.shape
+    _int32(page_table, "page_table", (B, most))
+    _int32(kv_lens, "kv_lens", (B,))
+    if cu_seqlens is not None:
+        _int32(cu_seqlens, "cu_seqlens", (B + 1,))
+        a.cu_seqlens = cu_seqlens.data_ptr()
+    elif tokens != B:
+        raise ValueError(f"{tokens} tokens of {B} sequences: without cu_seqlens there is one token per sequence")
+    a.B, a.max_pages = B, most
+    a.page_table, a.table_sb, a.kv_lens = page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr()
+
+
+def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, inv_freq, cu_seqlens=None, positions=None, pos_offset=0,
+                 q=None, q_weight=None, k_weight=None, eps=1e-6, q_out=None):
+    """Writes the keys (normed where ``k_weight`` is given, rotated) and values of new tokens into the pages of a cache;
+    with ``q`` the query heads are normed and rotated in the same launch.  k, v: (tokens, Hkv, D), q: (tokens, Hq, D);
+    pages: (num_pages, Hkv, page_size, D); page_table: (B, pages) int32; kv_lens: (B,) int32, the length of every
+    sequence with its new tokens; cu_seqlens: (B + 1,) int32, the first token of every sequence (None: one token each).
+    A token's position is ``pos_offset`` + its index in its sequence unless ``positions`` gives it.  Tokens behind the
+    last sequence, indices outside the table and page ids that name no page write nothing.  Returns the rotated
+    queries (``q_out`` if given; None without q)."""
+    _no_grad(k, v, q, q_weight, k_weight)
+    a = _lib.RopeArgs()
+    tokens, Hkv, D = _heads3(k, "k")
+    if _heads3(v, "v", k.dtype) != k.shape:
+        raise ValueError("k and v must have the same shape")
+    q_out = _rope_args(a, q, k, inv_freq, q_weight, k_weight, eps, q_out)
+    a.v, a.v_st, a.v_sh = v.data_ptr(), v.stride(0), v.stride(1)
+    _pages(a, k_pages, v_pages, k.dtype, Hkv, D)
+    _sequences(a, page_table, kv_lens, cu_seqlens, tokens)
+    if positions is not None:
+        _positions(a, positions, tokens)
+    a.pos_offset = pos_offset
+    _on(k.device, v, q, q_out, k_pages, v_pages, page_table, kv_lens, cu_seqlens, positions, inv_freq, q_weight,
+        k_weight)
+    _call(lib.fa_paged_append, "fa_paged_append", k.device, C.byref(a))
+    _count(1)
+    return q_out
+
+
+def paged_attention(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens=None, prefix_pages=None, prefix_len=0,
+                    sm_scale=None, out=None, return_lse=False):
+    """Attention of new tokens over the pages of their sequences and over a prefix that the whole batch shares, which is
+    read once for all of its rows.  q: (tokens, Hq, D), D 64 or 128, tokens packed as in :func:`paged_append`; the last
+    new token of sequence b sees ``kv_lens[b]`` keys of its own, each one before it a key less, and every token sees the
+    first ``prefix_len`` keys of ``prefix_pages`` (int32 page ids).  Returns (tokens, Hq, D) of q's dtype, with
+    ``return_lse`` also the log-sum-exp of the scores, (tokens, Hq) float32.  A token without any key gets 0 and
+    -infinity; tokens behind the last sequence are left as they were.  Scratch comes from PyTorch's allocator, per
+    call."""
+    _no_grad(q, k_pages, v_pages)
+    a = _lib.PagedAttnArgs()
+    a.dtype = _dt(q)
+    tokens, Hq, D = _heads3(q, "q")
+    if k_pages.dim() != 4:
+        raise ValueError("k_pages: expected (num_pages, kv_heads, page_size, head_dim)")
+    Hkv = k_pages.shape[1]
+    a.tokens, a.Hq, a.Hkv, a.D = tokens, Hq, Hkv, D
+    _pages(a, k_pages, v_pages, q.dtype, Hkv, D)
+    _sequences(a, page_table, kv_lens, cu_seqlens, tokens)
+    if prefix_len:
+        if prefix_pages is None or prefix_pages.dim() != 1:
+            raise ValueError("prefix_pages: expected an int32 vector of page ids")
+        _int32(prefix_pages, "prefix_pages", (prefix_pages.shape[0],))
+        a.prefix_pages, a.n_prefix_pages, a.prefix_len = prefix_pages.data_ptr(), prefix_pages.shape[0], prefix_len
+    a.sm_scale = -1.0 if sm_scale is None else sm_scale
+    if out is None:
+        out = torch.empty((tokens, Hq, D), dtype=q.dtype, device=q.device)
+    elif _heads3(out, "out", q.dtype) != q.shape:
+        raise ValueError("out must have the shape of q")
+    lse = torch.empty((tokens, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    a.q, a.q_st, a.q_sh = q.data_ptr(), q.stride(0), q.stride(1)
+    a.out, a.o_st, a.o_sh = out.data_ptr(), out.stride(0), out.stride(1)
+    a.lse = lse.data_ptr() if return_lse else None
+    _on(q.device, k_pages, v_pages, page_table, kv_lens, cu_seqlens, prefix_pages if prefix_len else None, out)
+    if tokens:
+        index = q.device.index
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(index):
+                return _paged_attention(a, q.device, out, lse, prefix_len)
+        return _paged_attention(a, q.device, out, lse, prefix_len)
+    return (out, lse) if return_lse else out
+
+
+def _paged_attention(a, dev, out, lse, prefix_len):
+    nbytes = lib.fa_paged_attn_scratch_bytes(C.byref(a))
+    if nbytes:
+        # of this call alone: a buffer kept between calls would be shared by captured graphs
+        sc = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        a.scratch, a.scratch_bytes = sc.data_ptr(), nbytes
+    rc = lib.fa_paged_attn(C.byref(a), torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        check(rc, "fa_paged_attn")
+    _count(3 if prefix_len else 2)
+    return out if lse is None else (out, lse)
+
+
+def _row_parameter(value, name, dtype, B):
+    """(pointer, value) of a per-row tensor or of one number for all rows."""
+    if isinstance(value, torch.Tensor):
+        if value.dtype != dtype or tuple(value.shape) != (B,) or not value.is_contiguous():
+            raise ValueError(f"{name}: expected a number or a contiguous {dtype} ({B},) tensor")
+        return value.data_ptr(), 0
+    return None, value
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_logprob=False):
+    """Draws one token per row of ``logits`` (B, V), float32, float16 or bfloat16, V <= 393216, with the uniform numbers
+    ``u`` (B,) float32 in [0, 1).  Temperature is applied first (0: the largest logit), then top-k (0: off), top-p on
+    what top-k kept (1: off), min-p relative to the largest probability (0: off); each is a number or a (B,) tensor
+    (float32, ``top_k`` int32).  Among equal logits the lower index counts as larger.  The token is the first index at
+    which the running sum of kept probabilities exceeds u.  Returns int64 tokens, with ``return_logprob`` also the
+    float32 logarithm of the probability each had in the kept distribution.  NaN logits are never drawn; a row without a
+    logit above -infinity gives token -1."""
+    _no_grad(logits)
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits: expected (B, V) with a contiguous last dimension")
+    B, V = logits.shape
+    dtype = _lib.FA_DTYPE_F32 if logits.dtype == torch.float32 else _dt(logits)
+    if u.dtype != torch.float32 or tuple(u.shape) != (B,) or not u.is_contiguous():
+        raise ValueError(f"u: expected a contiguous float32 ({B},) tensor")
+    tp, tv = _row_parameter(temperature, "temperature", torch.float32, B)
+    kp, kv = _row_parameter(top_k, "top_k", torch.int32, B)
+    pp, pv = _row_parameter(top_p, "top_p", torch.float32, B)
+    mp, mv = _row_parameter(min_p, "min_p", torch.float32, B)
+    dev = logits.device
+    _on(dev, u, *(t for t in (temperature, top_k, top_p, min_p) if isinstance(t, torch.Tensor)))
+    token = torch.empty((B,), dtype=torch.int64, device=dev)
+    logprob = torch.empty((B,), dtype=torch.float32, device=dev) if return_logprob else None
+    _call(lib.fa_sample, "fa_sample", dev, logits.data_ptr(), dtype, B, V, logits.stride(0), u.data_ptr(), tp, tv, kp, kv,
+          pp, pv, mp, mv, token.data_ptr(), logprob.data_ptr() if return_logprob else None)
+    _count(1)
+    return (token, logprob) if return_logprob else token
+
+
 def _count(n):
     global launch_count
     launch_count += n

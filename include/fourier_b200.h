@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-typedef enum { FA_DTYPE_F16 = 0, FA_DTYPE_BF16 = 1 } fa_dtype_t;
+typedef enum { FA_DTYPE_F16 = 0, FA_DTYPE_BF16 = 1, FA_DTYPE_F32 = 2 /* fa_sample only */ } fa_dtype_t;
 
 typedef enum {
   FA_OK = 0,
@@ -289,6 +289,89 @@ int fa_layer_decode_path(fa_layer_t* layer);
  * o: (n_parts, rows, D), m, l: (n_parts, rows). */
 int fa_merge(const float* o, const float* m, const float* l, int n_parts, int rows, int D,
              float* out, fa_stream_t stream);
+
+/* ---- a served batch outside the compressed span ---------------------------------------------------------
+ * The four calls below make the step of a batch of sequences of different lengths, from the projections to the
+ * token, over a cache of pages.  They have no counterpart in the reference, whose uncompressed sequences live in
+ * dense tensors grown by torch.cat (CU:681-686) and are attended by a library call (ML:627-633).
+ *
+ * Pages: (num_pages, Hkv, page_size, D), any strides with a contiguous last dimension.  Sequence b keeps its key j in
+ * row j % page_size of page page_table[b, j / page_size].  New tokens are packed: those of sequence b are the rows
+ * cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (ascending; without cu_seqlens every sequence has one), and kv_lens[b] is the
+ * number of its keys WITH them.  Rows behind the last sequence are left as they are.  Lengths, tables and positions are
+ * read on the device: a captured call follows them when it is replayed.
+ * A page id outside [0, num_pages) and an index outside the table hold no key: nothing is written there and nothing
+ * read. */
+typedef struct {
+  int32_t tokens, Hq, Hkv, D;
+  int32_t R;              /* rotary width, a multiple of 16 up to D: pairs (i, i + R/2), i < R/2            */
+  int32_t dtype;          /* of q, k, v, the outputs and the pages                                          */
+  int32_t w_f32;          /* the weights are float32 (else of `dtype`)                                      */
+  int32_t pos_i64;        /* `positions` is int64 (else int32)                                              */
+  const void *q, *k, *v;  /* (tokens, H*, D), strides *_st (token) and *_sh (head)                          */
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  void *q_out, *k_out;    /* may be the inputs                                                              */
+  int64_t qo_st, qo_sh, ko_st, ko_sh;
+  const void* positions;  /* (tokens)                                                                       */
+  const float* inv_freq;  /* (R/2): the angle of pair i is position * inv_freq[i]                           */
+  const void *q_weight, *k_weight; /* (D), or null: no norm                                                 */
+  float eps;
+  /* fa_paged_append */
+  int32_t B, page_size, max_pages, num_pages;
+  void *k_pages, *v_pages;
+  int64_t kp_sp, kp_sh, kp_sr, vp_sp, vp_sh, vp_sr; /* strides of page, head, row                           */
+  const int32_t* page_table;  /* (B, max_pages), row stride table_sb                                        */
+  int64_t table_sb;
+  const int32_t *kv_lens, *cu_seqlens;
+  int64_t pos_offset;     /* position of key 0 of every sequence (the length of a shared prefix)            */
+} fa_rope_args_t;
+
+/* q_out, k_out = the query and key heads, each divided by its root mean square and multiplied by its weight (where
+ * given), rotated by position.  Without norm this is apply_rotary_pos_emb (ML:263-286) in one launch, with exact
+ * angles and one rounding.  Hq or Hkv may be 0. */
+int fa_qk_norm_rope(const fa_rope_args_t* args_host, fa_stream_t stream);
+
+/* The same for q (Hq may be 0) and k, with k and v written to their pages.  positions may be null: then the position
+ * of a token is pos_offset + its index in its sequence. */
+int fa_paged_append(const fa_rope_args_t* args_host, fa_stream_t stream);
+
+typedef struct {
+  int32_t tokens, B, Hq, Hkv, D; /* D: 64 or 128                                                            */
+  int32_t page_size;      /* a multiple of 16                                                               */
+  int32_t num_pages, max_pages, n_prefix_pages, prefix_len, dtype;
+  float sm_scale;         /* softmax scale; <= 0 selects 1/sqrt(D)                                          */
+  const void* q;          /* (tokens, Hq, D); q, out and pages: 16-byte aligned, strides multiples of 8     */
+  int64_t q_st, q_sh;
+  void* out;              /* (tokens, Hq, D)                                                                */
+  int64_t o_st, o_sh;
+  float* lse;             /* (tokens, Hq) contiguous, natural logarithm, or null                            */
+  const void *k_pages, *v_pages;
+  int64_t kp_sp, kp_sh, kp_sr, vp_sp, vp_sh, vp_sr;
+  const int32_t* page_table;
+  int64_t table_sb;
+  const int32_t *kv_lens, *cu_seqlens;
+  const int32_t* prefix_pages; /* the pages of prefix_len keys that every token of the batch sees           */
+  void* scratch;          /* fa_paged_attn_scratch_bytes(), on 256 bytes                                    */
+  size_t scratch_bytes;
+} fa_paged_attn_args_t;
+
+/* Attention of the new tokens over the prefix (all of it) and their own sequence's keys up to themselves: the last new
+ * token sees kv_lens[b] keys, each one before it a key less.  The prefix is read once for the whole batch.  A row
+ * without keys gives 0, lse -infinity. */
+size_t fa_paged_attn_scratch_bytes(const fa_paged_attn_args_t* args_host);
+int fa_paged_attn(const fa_paged_attn_args_t* args_host, fa_stream_t stream);
+
+/* One token per row of logits (B, V), V <= 393216.  Weights w_i = exp((x_i - max x) / temperature), in the order
+ * "larger logit first, lower index first among equals"; kept are the first top_k of them (top_k <= 0: all), of those
+ * the shortest head whose weight reaches top_p times theirs (top_p >= 1: all), of those the ones of at least min_p
+ * times the largest.  The token is the first index whose running sum of kept weights (by index) exceeds u times their
+ * sum, 0 <= u < 1; logprob (or null) is the logarithm of its share.  temperature <= 0 takes the largest logit.  A NaN
+ * logit is never drawn; logits of +infinity share the probability; a row without a logit above -infinity gives
+ * token -1, logprob -infinity.  Every parameter is a (B) device array or, where that is null, the value next to it.
+ * Sums that decide are taken in float64 in a fixed order. */
+int fa_sample(const void* logits, int dtype, int B, int V, int64_t logits_sb, const float* u, const float* temperature,
+              float temperature0, const int32_t* top_k, int top_k0, const float* top_p, float top_p0, const float* min_p,
+              float min_p0, int64_t* token, float* logprob, fa_stream_t stream);
 
 #ifdef __cplusplus
 }
