@@ -12,6 +12,7 @@ import sys
 from . import _lib, ops  # noqa: F401  (fails loudly when the library has not been built)
 from . import cache_utils_fourier, fourier_triton_valid4_v2, modeling_llama_fourier  # noqa: F401
 from .cache_utils_fourier import DynamicCache, compress_period  # noqa: F401
+from .paged_cache import PagedCache  # noqa: F401
 
 __version__ = "0.1.0"
 

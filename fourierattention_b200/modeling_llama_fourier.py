@@ -14,7 +14,9 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as Fnn
 
+from . import ops
 from .cache_utils_fourier import Cache, DynamicCache, StaticCache  # noqa: F401  (re-exported names)
+from .paged_cache import PagedCache
 
 __all__ = ["LlamaConfig", "LlamaRMSNorm", "LlamaRotaryEmbedding", "LlamaMLP", "LlamaAttention",
            "LlamaSdpaAttention", "LLAMA_ATTENTION_CLASSES", "LlamaDecoderLayer", "LlamaModel", "LlamaForCausalLM",
@@ -22,12 +24,13 @@ __all__ = ["LlamaConfig", "LlamaRMSNorm", "LlamaRotaryEmbedding", "LlamaMLP", "L
 
 
 class LlamaConfig(SimpleNamespace):
-    """Attribute bag with Llama defaults (Llama-3.1-8B geometry)."""
+    """Attribute bag with Llama defaults (Llama-3.1-8B geometry).  ``qk_norm=True`` gives every attention layer
+    ``q_norm`` and ``k_norm``: an RMS norm of each query and key head before the rotation."""
 
     def __init__(self, **kw):
         d = dict(vocab_size=128256, hidden_size=4096, intermediate_size=14336, num_hidden_layers=32,
                  num_attention_heads=32, num_key_value_heads=8, head_dim=None, rms_norm_eps=1e-5,
-                 rope_theta=500000.0, max_position_embeddings=131072, attention_bias=False, mlp_bias=False,
+                 rope_theta=500000.0, max_position_embeddings=131072, attention_bias=False, mlp_bias=False, qk_norm=False,
                  initializer_range=0.02, _attn_implementation="sdpa")
         d.update(kw)
         if d["head_dim"] is None:
@@ -54,6 +57,11 @@ class LlamaRotaryEmbedding(nn.Module):
         dim = config.head_dim
         inv = 1.0 / (config.rope_theta ** (torch.arange(0, dim, 2, dtype=torch.float32) / dim))
         self.register_buffer("inv_freq", inv, persistent=False)
+
+    def frequencies(self):
+        """The frequencies as the fused operators take them: float32, with the values this module rotates with (a module
+        cast to float16 has rounded them)."""
+        return self.inv_freq.float()
 
     @torch.no_grad()
     def forward(self, x, position_ids):
@@ -101,6 +109,17 @@ class LlamaAttention(nn.Module):
         self.v_proj = nn.Linear(self.hidden_size, self.num_key_value_heads * self.head_dim, bias=b)
         self.o_proj = nn.Linear(self.num_heads * self.head_dim, self.hidden_size, bias=b)
         self.rotary_emb = LlamaRotaryEmbedding(config)
+        if getattr(config, "qk_norm", False):
+            self.q_norm = LlamaRMSNorm(self.head_dim, eps=config.rms_norm_eps)
+            self.k_norm = LlamaRMSNorm(self.head_dim, eps=config.rms_norm_eps)
+        else:
+            self.q_norm = self.k_norm = None
+
+    def _norm_args(self):
+        """The norm arguments of the fused operators."""
+        if self.q_norm is None:
+            return {}
+        return dict(q_weight=self.q_norm.weight, k_weight=self.k_norm.weight, eps=self.q_norm.variance_epsilon)
 
 
 def _dense_causal(q, k, v, num_kv_heads, head_dim):
@@ -129,14 +148,33 @@ class LlamaSdpaAttention(LlamaAttention):
         if output_attentions:
             raise NotImplementedError("output_attentions=True is not available on the Fourier path")
         bsz, q_len, _ = hidden_states.size()
-        q = self.q_proj(hidden_states).view(bsz, q_len, self.num_heads, self.head_dim).transpose(1, 2)
-        k = self.k_proj(hidden_states).view(bsz, q_len, self.num_key_value_heads, self.head_dim).transpose(1, 2)
-        v = self.v_proj(hidden_states).view(bsz, q_len, self.num_key_value_heads, self.head_dim).transpose(1, 2)
-        if position_embeddings is None:
-            cos, sin = self.rotary_emb(v, position_ids)
+        q, k, v = self.q_proj(hidden_states), self.k_proj(hidden_states), self.v_proj(hidden_states)
+        if isinstance(past_key_value, PagedCache):
+            rows = lambda x: x.view(bsz * q_len, -1, self.head_dim)
+            attn = past_key_value.attend(rows(q), rows(k), rows(v), self.layer_idx, self.rotary_emb.frequencies(),
+                                         positions=None if position_ids is None else
+                                         position_ids.expand(bsz, q_len).reshape(-1).contiguous(),
+                                         **self._norm_args())
+            return self.o_proj(attn.view(bsz, q_len, -1)), None, past_key_value
+        q = q.view(bsz, q_len, self.num_heads, self.head_dim).transpose(1, 2)
+        k = k.view(bsz, q_len, self.num_key_value_heads, self.head_dim).transpose(1, 2)
+        v = v.view(bsz, q_len, self.num_key_value_heads, self.head_dim).transpose(1, 2)
+        if self.q_norm is not None:
+            cos, sin = position_embeddings or (None, None)
+            # norm and rotation in one pass, from the positions themselves
+            if position_ids is None:
+                raise ValueError("qk_norm layers need position_ids")
+            rows = lambda x: x.transpose(1, 2).reshape(bsz * q_len, -1, self.head_dim)
+            q, k = ops.qk_norm_rope(rows(q), rows(k), position_ids.expand(bsz, q_len).reshape(-1).contiguous(),
+                                    self.rotary_emb.frequencies(), **self._norm_args())
+            q = q.view(bsz, q_len, self.num_heads, self.head_dim).transpose(1, 2)
+            k = k.view(bsz, q_len, self.num_key_value_heads, self.head_dim).transpose(1, 2)
         else:
-            cos, sin = position_embeddings
-        q, k = apply_rotary_pos_emb(q, k, cos, sin)
+            if position_embeddings is None:
+                cos, sin = self.rotary_emb(v, position_ids)
+            else:
+                cos, sin = position_embeddings
+            q, k = apply_rotary_pos_emb(q, k, cos, sin)
 
         if past_key_value is None:
             kd = {"k_init": None, "k_compressed": None, "k_uncompressed": None,
@@ -202,13 +240,19 @@ class LlamaModel(nn.Module):
 
     def forward(self, input_ids, past_key_values=None, position_ids=None, use_cache=True):
         h = self.embed_tokens(input_ids)
+        if isinstance(past_key_values, PagedCache):
+            # positions follow from the cache's lengths, and rotation happens where the keys are stored
+            past_key_values.begin_step(*input_ids.shape)
+            for layer in self.layers:
+                h = layer(h, past_key_value=past_key_values, position_ids=position_ids)
+            return self.norm(h)
         if position_ids is None:
             past = past_key_values._seen_tokens if past_key_values is not None else 0
             position_ids = torch.arange(past, past + input_ids.shape[1], device=input_ids.device)[None].expand(
                 input_ids.shape[0], -1)
         pe = self.rotary_emb(h, position_ids)
         for layer in self.layers:
-            h = layer(h, past_key_value=past_key_values, position_embeddings=pe)
+            h = layer(h, past_key_value=past_key_values, position_embeddings=pe, position_ids=position_ids)
         return self.norm(h)
 
 
@@ -227,5 +271,30 @@ class LlamaForCausalLM(nn.Module):
 
     def forward(self, input_ids, past_key_values=None, use_cache=True, num_logits_to_keep: int = 1, **kwargs):
         h = self.model(input_ids, past_key_values=past_key_values)
+        if isinstance(past_key_values, PagedCache) and num_logits_to_keep == 1:
+            h = past_key_values.last_rows(h)                 # of every sequence, packed or not
         logits = self.lm_head(h[:, -num_logits_to_keep:, :])
         return SimpleNamespace(logits=logits, past_key_values=past_key_values)
+
+    @torch.no_grad()
+    def generate(self, input_ids, past_key_values, max_new_tokens: int, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                 uniform=None, generator=None, eos_token_id: Optional[int] = None):
+        """Runs the prompt (``input_ids`` as :meth:`forward` takes them) and draws ``max_new_tokens`` tokens per sequence
+        with ``ops.sample`` (its parameters: numbers or one value per sequence; ``temperature=0`` is greedy).
+        ``uniform``: (batch, max_new_tokens) float32 in [0, 1), drawn with ``generator`` if not given.  Tokens behind
+        ``eos_token_id`` are ``eos_token_id``.  Returns (batch, max_new_tokens) int64; the last token drawn is not in the
+        cache yet."""
+        tokens, done = [], None
+        for i in range(max_new_tokens):
+            logits = self(input_ids, past_key_values=past_key_values).logits[:, -1]
+            if uniform is None:
+                uniform = torch.rand((logits.shape[0], max_new_tokens), device=logits.device, generator=generator)
+            token = ops.sample(logits, uniform[:, i].contiguous(), temperature=temperature, top_k=top_k, top_p=top_p,
+                               min_p=min_p)
+            if eos_token_id is not None:
+                if done is not None:
+                    token = torch.where(done, eos_token_id, token)
+                done = token == eos_token_id
+            tokens.append(token)
+            input_ids = token[:, None]
+        return torch.stack(tokens, dim=1) if tokens else torch.empty((0, 0), dtype=torch.int64, device=input_ids.device)
