@@ -2,7 +2,7 @@
 //   row (token, query head):  s_j = scale q . k_j,  m = max s,  p_j = e^(s_j - m),  l = sum p,  o = sum p_j v_j / l,
 //   lse = m + ln l;  the keys are all of the prefix and the sequence's own keys up to the token.  A row without keys
 //   gives o = 0, lse = -inf.
-#include "paged_attn.cuh"
+#include "paged_tile.cuh"
 
 namespace fa {
 
@@ -433,23 +433,24 @@ static PaPlan pa_plan(const fa_paged_attn_args_t* a) {
   PaPlan pl;
   const int64_t G = a->Hq / a->Hkv;
   pl.ctas = sm_count();
-  // eight rows fill the streaming kernel's instruction; sixteen take a second one per key
-  pl.rows_own = (a->cu_seqlens ? G * 2 : G) <= 8 ? 8 : 16;
-  pl.rows_pre = (int64_t)a->tokens * G <= 8 ? 8 : 16;
+  // eight rows fill the streaming kernel's instruction; sixteen take a second one per key; more go to the tile kernel
+  const int64_t own = a->cu_seqlens ? (int64_t)a->tokens * G / a->B : G, pre = (int64_t)a->tokens * G;
+  pl.rows_own = a->cu_seqlens && own > 16 ? PT_ROWS : own <= 8 ? 8 : 16;
+  pl.rows_pre = pre > 16 ? PT_ROWS : pre <= 8 ? 8 : 16;
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t r = at;
     at += (n + 255) / 256 * 256;
     return r;
   };
-  const bool pre = a->prefix_len > 0;
-  for (int i = 0; i < (pre ? 2 : 1); ++i) {
+  const bool shared = a->prefix_len > 0;
+  for (int i = 0; i < (shared ? 2 : 1); ++i) {
     const int64_t rows = i == 0 ? pl.rows_own : pl.rows_pre;
     pl.slot_o[i] = take((size_t)2 * pl.ctas * rows * a->D * 4);
     pl.slot_ml[i] = take((size_t)2 * pl.ctas * rows * 8);
     pl.info[i] = take((size_t)pa_info_count(a->tokens, i == 0 ? a->B : 1, G, a->Hkv, rows) * 8);
     pl.row_o[i] = pl.row_ml[i] = 0;
-    if (pre) {
+    if (shared) {
       pl.row_o[i] = take((size_t)a->tokens * a->Hq * a->D * 4);
       pl.row_ml[i] = take((size_t)a->tokens * a->Hq * 8);
     }
@@ -469,6 +470,16 @@ static int pa_stream_launch(const PaStreamParams& prm, cudaStream_t st) {
 }
 
 template <typename T, int D>
+static int pa_tile_launch(const PaTileParams& prm, cudaStream_t st) {
+  constexpr int smem = PaTile<D>::SMEM;
+  cudaError_t e = cudaFuncSetAttribute(paged_tile_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_tile)");
+  paged_tile_kernel<T, D><<<prm.p.ctas, PT_THREADS, smem, st>>>(prm);
+  FA_CHECK_LAUNCH("fa_paged_attn(tile)");
+  return FA_OK;
+}
+
+template <typename T, int D>
 static int pa_run(const fa_paged_attn_args_t* a, cudaStream_t st) {
   const PaPlan pl = pa_plan(a);
   unsigned char* s = reinterpret_cast<unsigned char*>(a->scratch);
@@ -482,9 +493,21 @@ static int pa_run(const fa_paged_attn_args_t* a, cudaStream_t st) {
   c.page_size = a->page_size, c.num_pages = a->num_pages;
   const float scale = a->sm_scale > 0.f ? a->sm_scale : 1.f / sqrtf((float)D);
   c.scale_log2 = scale * 1.4426950408889634f;
-  int rc = pa_map(&prm.tm_k, a->k_pages, a, a->kp_sp, a->kp_sh, a->kp_sr, 16);
-  if (rc == FA_OK) rc = pa_map(&prm.tm_v, a->v_pages, a, a->vp_sp, a->vp_sh, a->vp_sr, 16);
+  const bool shared = a->prefix_len > 0;
+  PaTileParams tile;
+  tile.box_rows = 16;
+  while (tile.box_rows < PA_TILE && a->page_size % (2 * tile.box_rows) == 0) tile.box_rows *= 2;
+  int rc = FA_OK;
+  if (pl.rows_own < PT_ROWS || (shared && pl.rows_pre < PT_ROWS)) {
+    rc = pa_map(&prm.tm_k, a->k_pages, a, a->kp_sp, a->kp_sh, a->kp_sr, 16);
+    if (rc == FA_OK) rc = pa_map(&prm.tm_v, a->v_pages, a, a->vp_sp, a->vp_sh, a->vp_sr, 16);
+  }
+  if (rc == FA_OK && (pl.rows_own == PT_ROWS || (shared && pl.rows_pre == PT_ROWS))) {
+    rc = pa_map(&tile.tm_k, a->k_pages, a, a->kp_sp, a->kp_sh, a->kp_sr, tile.box_rows);
+    if (rc == FA_OK) rc = pa_map(&tile.tm_v, a->v_pages, a, a->vp_sp, a->vp_sh, a->vp_sr, tile.box_rows);
+  }
   if (rc != FA_OK) return rc;
+  tile.c = c;
   PaMergeParams mg;
   mg.c = c;
   auto phase = [&](int i) {
@@ -495,7 +518,7 @@ static int pa_run(const fa_paged_attn_args_t* a, cudaStream_t st) {
     p.prefix_len = i == 0 ? 0 : a->prefix_len;
     p.rows = i == 0 ? pl.rows_own : pl.rows_pre;
     p.ctas = pl.ctas;
-    p.direct = a->prefix_len == 0;
+    p.direct = !shared;
     p.slot_o = reinterpret_cast<float*>(s + pl.slot_o[i]);
     p.slot_ml = reinterpret_cast<float2*>(s + pl.slot_ml[i]);
     p.row_o = reinterpret_cast<float*>(s + pl.row_o[i]);
@@ -504,10 +527,12 @@ static int pa_run(const fa_paged_attn_args_t* a, cudaStream_t st) {
     return p;
   };
   mg.prefix.prefix_len = 0;
-  for (int i = a->prefix_len > 0 ? 1 : 0; i >= 0; --i) {
-    prm.p = phase(i);
+  for (int i = shared ? 1 : 0; i >= 0; --i) {
+    prm.p = tile.p = phase(i);
     (i == 0 ? mg.own : mg.prefix) = prm.p;
-    rc = prm.p.rows == 8 ? pa_stream_launch<T, D, 1>(prm, st) : pa_stream_launch<T, D, 2>(prm, st);
+    rc = prm.p.rows == PT_ROWS ? pa_tile_launch<T, D>(tile, st)
+         : prm.p.rows == 8     ? pa_stream_launch<T, D, 1>(prm, st)
+                               : pa_stream_launch<T, D, 2>(prm, st);
     if (rc != FA_OK) return rc;
   }
   const int64_t rows = (int64_t)a->tokens * a->Hq;

@@ -1,0 +1,435 @@
+// Many query rows per key: the tensor-core form of the paged attention.
+//
+// A unit is up to 256 query rows (two tiles of 128) that read the same keys.  Per 128-key tile and query tile
+//   S = Q K^T   (tcgen05.mma, both from shared memory, M = N = 128),  P = 2^(S - m) rounded to the cache's type,
+//   O += P V    (tcgen05.mma, P from tensor memory, V as it lies in the page: the MN-major operand).
+// Bound: the tensor pipe (2 x 512 cycles per query tile and key tile at D = 128) and the exponentials (16 per cycle and
+// SM: 1024 cycles), which run side by side: two warpgroups, one per query tile, take turns with the tensor pipe.
+//   warps 0-3, 4-7   softmax of query tile 0 / 1, a row per thread: no shuffles, running maximum in a register
+//   warp 8           issues the MMAs (one lane), owns tensor memory
+//   warp 9           fetches K and V tiles by TMA, a page's rows at a time, into a ring of 32 KB slots
+//   warps 10, 11     complete the warpgroup that gives its registers away
+// Tensor memory (512 columns): S0, S1 (128 each; P overwrites the first half of its S), O0, O1.  MMAs execute in the order
+// of their issue, so S of the next tile may be issued behind the product that still reads P.  The running maximum moves
+// only when a row passes it by 2^8; then the row's thread rescales its accumulator in tensor memory, which nothing else
+// touches at that point: the product before has completed (the commit that announced S covers it), the next one waits
+// for P.
+#pragma once
+
+#include "paged_attn.cuh"
+
+namespace fa {
+
+constexpr int PT_THREADS = 384;                          // 168 registers each at launch, moved to where they are needed:
+constexpr int PT_SOFTMAX_REGS = 216, PT_OTHER_REGS = 72;   // 256 x 216 + 128 x 72 = 384 x 168
+constexpr int PT_ROWS = 256;
+
+template <int D>
+struct PaTile {
+  static constexpr int HALF = 128 * 128;                  // 128 rows x 64 columns
+  static constexpr int SLOT = (D / 64) * HALF;            // a K or V tile
+  static constexpr int QBYTES = 2 * SLOT;
+  static constexpr int ST = 160 * 1024 / SLOT;            // 5 slots at D = 128
+  struct Small {
+    uint64_t full[ST], empty[ST], q_full[2], s_full[2], p_full[2], o_full[2], tail;
+    uint32_t bad[16];          // keys of a tile that no page holds, by groups of 16; the fetches are < 16 tiles ahead
+    PaLocate loc;
+    uint32_t tmem;
+    int dead;
+  };
+  static constexpr int SMEM = QBYTES + ST * SLOT + 1024;
+  static_assert(sizeof(Small) <= 1024, "barriers");
+};
+
+struct PaTileParams {
+  alignas(64) CUtensorMap tm_k, tm_v;
+  PaCommon c;
+  PaPhase p;
+  int box_rows;                // rows of a TMA box: a power of two that divides the page
+};
+
+// shared-memory matrix descriptors, 128-byte swizzle: start address, leading and stride byte offsets in 16-byte units
+__device__ __forceinline__ uint64_t pt_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) |
+         ((uint64_t)((sbo >> 4) & 0x3FFF) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc) : "memory");
+}
+__device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc) : "memory");
+}
+__device__ __forceinline__ void pt_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void pt_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void pt_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+#define PT_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define PT_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+// 32 columns of this warp's 32 lanes; the values are there after pt_wait_ld()
+__device__ __forceinline__ void pt_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      : PT_R8(r, 0), PT_R8(r, 8), PT_R8(r, 16), PT_R8(r, 24) : "r"(taddr));
+}
+__device__ __forceinline__ void pt_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void pt_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(taddr),
+      PT_W8(r, 0), PT_W8(r, 8), PT_W8(r, 16), PT_W8(r, 24) : "memory");
+}
+__device__ __forceinline__ void pt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+
+template <typename T>
+struct PtFormat;
+template <>
+struct PtFormat<__half> {
+  static constexpr uint32_t F = 0;
+};
+template <>
+struct PtFormat<__nv_bfloat16> {
+  static constexpr uint32_t F = 1;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_constant__ PaTileParams prm) {
+  using C = PaTile<D>;
+  const PaCommon& c = prm.c;
+  const PaPhase& p = prm.p;
+  extern __shared__ __align__(1024) unsigned char pa_dyn[];
+  typename C::Small& sh = *reinterpret_cast<typename C::Small*>(pa_dyn + C::QBYTES + C::ST * C::SLOT);
+  const uint32_t q_smem = pa_smem(pa_dyn), ring = q_smem + C::QBYTES;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  volatile int* dead = &sh.dead;
+
+  if (tid == 0) {
+    sh.dead = (q_smem & 1023u) ? 1 : 0;                   // the swizzle pattern goes by the address
+    for (int s = 0; s < C::ST; ++s) {
+      pa_bar_init(pa_smem(&sh.full[s]), 1);
+      pa_bar_init(pa_smem(&sh.empty[s]), 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      pa_bar_init(pa_smem(&sh.q_full[w]), 128);
+      pa_bar_init(pa_smem(&sh.s_full[w]), 1);
+      pa_bar_init(pa_smem(&sh.p_full[w]), 128);
+      pa_bar_init(pa_smem(&sh.o_full[w]), 1);
+    }
+    pa_bar_init(pa_smem(&sh.tail), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(pa_smem(&sh.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  pt_before();
+  PaUnit u;
+  int t;
+  const PaRange range = pa_locate<PT_THREADS>(c, p, blockIdx.x, sh.loc, u, t);   // two block barriers
+  pt_after();
+  const uint32_t tmem = sh.tmem;
+  long long done = range.beg;
+
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(PT_SOFTMAX_REGS));
+    // ---- softmax ------------------------------------------------------------------------------------------------------
+    const int w = warp >> 2, i = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + w * 128 + lanes, to = tmem + 256 + w * 128 + lanes;
+    const uint32_t s_full = pa_smem(&sh.s_full[w]), p_full = pa_smem(&sh.p_full[w]);
+    uint32_t s_par = 0, o_par = 0;
+    int tile_no = 0;                                      // tiles since the start
+    while (done < range.end) {
+      if (t >= u.tiles) {
+        u.next(c, p);
+        t = 0;
+        continue;
+      }
+      const int t_end = (int)min((long long)u.tiles, t + (range.end - done));
+      const int row0 = u.rb * PT_ROWS + w * 128;
+      const long long all_rows = (long long)u.s.n * c.G;
+      const int n_rows = (int)max(0LL, min(128LL, all_rows - row0));
+      if (n_rows == 0) {
+        tile_no += t_end - t;
+      } else {
+        // the query tile, zeros behind the last row
+        const uint32_t qb = q_smem + w * C::SLOT;
+#pragma unroll 4
+        for (int e = i; e < 128 * (D / 8); e += 128) {
+          const int r = e / (D / 8), ch = e % (D / 8);
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (r < n_rows) {
+            const int tok = (row0 + r) / c.G, hg = (row0 + r) - tok * c.G;
+            v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(c.q) + (int64_t)(u.s.t0 + tok) * c.q_st +
+                                                (int64_t)(u.h * c.G + hg) * c.q_sh + ch * 8);
+          }
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(qb + (ch >> 3) * C::HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
+                       "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // generic writes -> MMA reads
+        pt_before();
+        pa_bar_arrive(pa_smem(&sh.q_full[w]));
+
+        const int my_tok = (int)min((long long)row0 + i, all_rows - 1);
+        const int lim = p.prefix_len > 0 ? u.s.L : min(u.s.L, u.s.L - u.s.n + my_tok / c.G + 1);
+        float m = -INFINITY, l = 0.f;
+        for (int tt = t; tt < t_end; ++tt) {
+          pa_bar_wait(s_full, s_par, dead);
+          s_par ^= 1;
+          pt_after();
+          uint32_t sr[128];
+          pt_ld32(ts, sr);
+          pt_ld32(ts + 32, sr + 32);
+          pt_ld32(ts + 64, sr + 64);
+          pt_ld32(ts + 96, sr + 96);
+          pt_wait_ld();
+          float* s = reinterpret_cast<float*>(sr);
+          const uint32_t bad = sh.bad[tile_no++ & 15];
+          const int nv = lim - tt * PA_TILE;              // keys of the tile this row sees
+          if (__any_sync(0xffffffffu, nv < PA_TILE || bad != 0)) {
+#pragma unroll
+            for (int j = 0; j < 128; ++j)
+              if (j >= nv || ((bad >> (j / 16)) & 1)) s[j] = -INFINITY;
+          }
+          float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c.scale_log2;
+          if (__any_sync(0xffffffffu, top > m + 8.f)) {
+            const float nm = fmaxf(m, top);
+            const float f = m == -INFINITY ? 0.f : pa_ex2(m - nm);
+            m = nm;
+            l *= f;
+            if (tt > t) {
+#pragma unroll
+              for (int j = 0; j < D; j += 32) {
+                uint32_t o[32];
+                pt_ld32(to + j, o);
+                pt_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                pt_st32(to + j, o);
+              }
+            }
+          }
+          const float off = m == -INFINITY ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 128; ++j) {
+            s[j] = pa_ex2(fmaf(s[j], c.scale_log2, -off));
+            sum[j & 3] += s[j];
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+          for (int j = 0; j < 64; ++j) sr[j] = pa_pack<T>(s[2 * j], s[2 * j + 1]);
+          pt_st32(ts, sr);
+          pt_st32(ts + 32, sr + 32);
+          pt_wait_st();
+          pt_before();
+          pa_bar_arrive(p_full);
+        }
+        // ---- this segment's result ------------------------------------------------------------------------------------
+        pa_bar_wait(pa_smem(&sh.o_full[w]), o_par, dead);
+        o_par ^= 1;
+        pt_after();
+        const bool first = t == 0, last = t_end == u.tiles, whole = first && last;
+        if (*dead) l = __int_as_float(0x7fc00000);
+        const int r = row0 + i;
+        const int tok = u.s.t0 + r / c.G, hq = u.h * c.G + r % c.G;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int j = 0; j < D; j += 32) {
+          uint32_t o[32];
+          pt_ld32(to + j, o);
+          pt_wait_ld();
+          if (i >= n_rows) continue;
+          if (whole && p.direct) {
+            uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(c.out) + (int64_t)tok * c.o_st + (int64_t)hq * c.o_sh + j);
+            uint32_t v[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] = pa_pack<T>(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) dst[k] = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+          } else {
+            const int64_t at = whole ? (int64_t)tok * c.Hq + hq : (int64_t)(2 * blockIdx.x + (first ? 1 : 0)) * PT_ROWS + w * 128 + i;
+            uint4* dst = reinterpret_cast<uint4*>((whole ? p.row_o : p.slot_o) + at * D + j);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) dst[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          }
+        }
+        if (i < n_rows) {
+          if (whole && p.direct) {
+            if (c.lse) c.lse[(int64_t)tok * c.Hq + hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+          } else {
+            const int64_t at = whole ? (int64_t)tok * c.Hq + hq : (int64_t)(2 * blockIdx.x + (first ? 1 : 0)) * PT_ROWS + w * 128 + i;
+            (whole ? p.row_ml : p.slot_ml)[at] = make_float2(m, l);
+          }
+        }
+        pt_before();
+        if (last && w == 0 && i == 0)
+          p.info[pa_unit_id(c, p, u.b, u.s, u.h, u.rb)] = make_int2(pa_owner(range, done - t), blockIdx.x);
+      }
+      done += t_end - t;
+      t = t_end;
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PT_OTHER_REGS));
+  }
+  if (warp == 8) {
+    // ---- the MMAs -----------------------------------------------------------------------------------------------------
+    constexpr uint32_t F = PtFormat<T>::F;
+    const uint32_t id_qk = (1u << 4) | (F << 7) | (F << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    const uint32_t id_pv = (1u << 4) | (F << 7) | (F << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
+    int slot = 0;
+    uint32_t par = 0, q_par = 0, p_par = 0;               // q_par, p_par: a bit per query tile
+    while (done < range.end) {
+      if (t >= u.tiles) {
+        u.next(c, p);
+        t = 0;
+        continue;
+      }
+      const int t_end = (int)min((long long)u.tiles, t + (range.end - done));
+      const int nw = (long long)u.s.n * c.G - (long long)u.rb * PT_ROWS > 128 ? 2 : 1;
+      auto scores = [&](int w, uint32_t kb) {
+        if (lane == 0) {
+          const uint32_t qb = q_smem + w * C::SLOT;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t o = (kk >> 2) * C::HALF + (kk & 3) * 32;
+            pt_mma_ss(tmem + w * 128, pt_desc(qb + o, 16, 1024), pt_desc(kb + o, 16, 1024), id_qk, kk > 0);
+          }
+          pt_commit(pa_smem(&sh.s_full[w]));
+        }
+        __syncwarp();
+      };
+      auto advance = [&]() {
+        if (++slot == C::ST) slot = 0, par ^= 1;
+      };
+      // K of the first tile
+      pa_bar_wait(pa_smem(&sh.full[slot]), par, dead);
+      for (int w = 0; w < nw; ++w) {
+        pa_bar_wait(pa_smem(&sh.q_full[w]), (q_par >> w) & 1, dead);
+        q_par ^= 1u << w;
+        pt_after();
+        scores(w, ring + slot * C::SLOT);
+      }
+      if (lane == 0) pt_commit(pa_smem(&sh.empty[slot]));
+      __syncwarp();
+      advance();
+      for (int tt = t; tt < t_end; ++tt) {
+        const bool more = tt + 1 < t_end;
+        const int nv = min(PA_TILE, u.limit - tt * PA_TILE), steps = (nv + 15) / 16;
+        const int v_slot = slot;
+        const uint32_t vb = ring + slot * C::SLOT;
+        pa_bar_wait(pa_smem(&sh.full[slot]), par, dead);
+        advance();
+        const int k_slot = slot;
+        if (more) {
+          pa_bar_wait(pa_smem(&sh.full[slot]), par, dead);
+          advance();
+        }
+        for (int w = 0; w < nw; ++w) {
+          pa_bar_wait(pa_smem(&sh.p_full[w]), (p_par >> w) & 1, dead);
+          p_par ^= 1u << w;
+          pt_after();
+          if (lane == 0) {
+            for (int kk = 0; kk < steps; ++kk)
+              pt_mma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8, pt_desc(vb + kk * 2048, C::HALF, 1024), id_pv,
+                        tt > t || kk > 0);
+            if (!more) pt_commit(pa_smem(&sh.o_full[w]));
+          }
+          __syncwarp();
+          if (more) scores(w, ring + k_slot * C::SLOT);
+        }
+        if (lane == 0) {
+          pt_commit(pa_smem(&sh.empty[v_slot]));
+          if (more) pt_commit(pa_smem(&sh.empty[k_slot]));
+        }
+        __syncwarp();
+      }
+      done += t_end - t;
+      t = t_end;
+    }
+  } else if (warp == 9) {
+    // ---- the fetches --------------------------------------------------------------------------------------------------
+    int slot = 0, tile_no = 0;
+    uint32_t par = 1, t_par = 0;                          // the first pass over the ring finds it empty
+    const int n_box = PA_TILE / prm.box_rows;
+    const uint32_t box_bytes = prm.box_rows * 128;
+    while (done < range.end) {
+      if (t >= u.tiles) {
+        u.next(c, p);
+        t = 0;
+        continue;
+      }
+      const int key0 = t * PA_TILE, nv = min(PA_TILE, u.limit - key0);
+      const int need = (nv + prm.box_rows - 1) / prm.box_rows;        // boxes with keys
+      int page = c.num_pages, row = 0;
+      bool ok = true;
+      if (lane < need) {
+        const int key = key0 + lane * prm.box_rows;
+        page = p.table[(int64_t)u.b * p.table_sb + key / c.page_size];
+        row = key % c.page_size;
+        ok = page >= 0 && page < c.num_pages;
+        if (!ok) page = c.num_pages;                      // out of the map's range: zeros arrive
+      }
+      // groups of 16 keys whose page id names no page
+      const uint32_t miss = __ballot_sync(0xffffffffu, !ok);
+      uint32_t bad = 0;
+      for (int b = 0; b < n_box; ++b)
+        if ((miss >> b) & 1)
+          for (int g = b * (prm.box_rows / 16); g < (b + 1) * (prm.box_rows / 16); ++g) bad |= 1u << g;
+      const bool tail = key0 + PA_TILE > u.s.L && (u.s.L & 15);        // keys and leftovers in one group of 16
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint32_t dst = ring + slot * C::SLOT, full = pa_smem(&sh.full[slot]);
+        const uint32_t bar = kv == 1 && tail ? pa_smem(&sh.tail) : full;
+        pa_bar_wait(pa_smem(&sh.empty[slot]), par, dead);
+        if (lane == 0) {
+          if (kv == 0) sh.bad[tile_no & 15] = bad;
+          pa_bar_expect(bar, (uint32_t)need * box_bytes * (D / 64));
+        }
+        __syncwarp();
+        if (lane < need)
+          for (int hf = 0; hf < D / 64; ++hf)
+            pa_tma(dst + hf * C::HALF + lane * box_bytes, kv == 0 ? &prm.tm_k : &prm.tm_v, 64 * hf, row, u.h, page, bar);
+        if (kv == 1 && tail) {
+          // rows behind the sequence hold anything, and 0 x NaN must not reach the sums: zeros up to the end of the
+          // group of 16 (the product stops there)
+          pa_bar_wait(bar, t_par, dead);
+          t_par ^= 1;
+          const int r0 = u.s.L - key0, r1 = (r0 + 15) & ~15;
+          for (int e = lane; e < (r1 - r0) * (D / 8); e += 32) {
+            const int r = r0 + e / (D / 8), ch = e % (D / 8);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(dst + (ch >> 3) * C::HALF + r * 128 + ((ch & 7) << 4)), "r"(0) : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+          __syncwarp();
+          if (lane == 0) pa_bar_arrive(full);
+        }
+        if (++slot == C::ST) slot = 0, par ^= 1;
+      }
+      ++done, ++t, ++tile_no;
+    }
+  }
+  if (*dead) {
+    // a wait gave up: leave time for what is still in flight
+    const long long t0 = clock64();
+    while (clock64() - t0 < 20000000LL) __nanosleep(1000);
+  }
+  pt_before();
+  __syncthreads();
+  if (warp == 8) {
+    pt_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+  }
+}
+
+}  // namespace fa
