@@ -342,15 +342,26 @@ struct PaMergeParams {
   PaPhase own, prefix;       // prefix.prefix_len == 0: none
 };
 
+// One part into the running sums.
 template <int D>
-__device__ __forceinline__ void pa_take(float2 ml, const float* o, int lane, float& m, float& l, float* acc) {
+__device__ __forceinline__ void pa_take(float2 ml, const float* o, float& m, float& l, float* acc) {
   const float mx = fmaxf(m, ml.x);
   if (mx == -INFINITY) return;
   const float f0 = pa_ex2(m - mx), f1 = pa_ex2(ml.x - mx);
   l = l * f0 + ml.y * f1;
   m = mx;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = acc[i] * f0 + o[lane * (D / 32) + i] * f1;
+  for (int i = 0; i < D / 32; ++i) acc[i] = acc[i] * f0 + o[i] * f1;
+}
+template <int D>
+__device__ __forceinline__ void pa_load(const float* src, int lane, float* o) {
+  if (D == 128) {
+    const float4 v = *reinterpret_cast<const float4*>(src + 4 * lane);
+    o[0] = v.x, o[1] = v.y, o[2] = v.z, o[D / 32 - 1] = v.w;
+  } else {
+    const float2 v = *reinterpret_cast<const float2*>(src + 2 * lane);
+    o[0] = v.x, o[1] = v.y;
+  }
 }
 
 template <typename T, int D>
@@ -381,11 +392,25 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
     const int2 who = p.info[pa_unit_id(c, p, pb, s, h, rb)];
     if (who.x == who.y) {
       if (p.direct) return;               // already written
-      pa_take<D>(p.row_ml[row], p.row_o + row * D, lane, m, l, acc);
+      float o[D / 32];
+      pa_load<D>(p.row_o + row * D, lane, o);
+      pa_take<D>(p.row_ml[row], o, m, l, acc);
     } else {
-      for (int cta = who.x; cta <= who.y; ++cta) {
-        const int64_t at = (int64_t)(2 * cta + (cta == who.x ? 1 : 0)) * p.rows + (r - (long long)rb * p.rows);
-        pa_take<D>(p.slot_ml[at], p.slot_o + at * D, lane, m, l, acc);
+      // eight parts are requested before the first is used
+      const int64_t in_block = r - (long long)rb * p.rows;
+      for (int cta = who.x; cta <= who.y; cta += 8) {
+        float o[8][D / 32];
+        float2 ml[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (cta + k > who.y) break;
+          const int64_t at = (int64_t)(2 * (cta + k) + (cta + k == who.x ? 1 : 0)) * p.rows + in_block;
+          ml[k] = p.slot_ml[at];
+          pa_load<D>(p.slot_o + at * D, lane, o[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (cta + k <= who.y) pa_take<D>(ml[k], o[k], m, l, acc);
       }
     }
   }

@@ -4,25 +4,42 @@
 //   S = Q K^T   (tcgen05.mma, both from shared memory, M = N = 128),  P = 2^(S - m) rounded to the cache's type,
 //   O += P V    (tcgen05.mma, P from tensor memory, V as it lies in the page: the MN-major operand).
 // Bound: the tensor pipe (2 x 512 cycles per query tile and key tile at D = 128) and the exponentials (16 per cycle and
-// SM: 1024 cycles), which run side by side: two warpgroups, one per query tile, take turns with the tensor pipe.
-//   warps 0-3, 4-7   softmax of query tile 0 / 1, a row per thread: no shuffles, running maximum in a register
-//   warp 8           issues the MMAs (one lane), owns tensor memory
-//   warp 9           fetches K and V tiles by TMA, a page's rows at a time, into a ring of 32 KB slots
-//   warps 10, 11     complete the warpgroup that gives its registers away
+// SM: 1024 cycles), which run side by side: the warps of one query tile work while the other's products run.
+//   warps 0-7, 8-15  softmax of query tile 0 / 1: two threads per row, 64 keys each.  One thread per row with 128 keys
+//                    took 4900 cycles per key tile, bound by the latency of a lone warp per scheduler and tile; four
+//                    warps per scheduler cover it.  The two halves agree through one barrier with a vote.
+//   warp 16          issues the MMAs and owns tensor memory.  The issuing lane is chosen by elect.sync, descriptors are
+//                    made once: the operands then sit in uniform registers and an MMA takes ~20 cycles to issue; behind
+//                    `lane == 0`, with descriptors made per MMA, it took 100 to 160 and bound the kernel (an MMA of
+//                    128 x 128 x 16 runs 64)
+//   warp 17          fetches K and V tiles by TMA, a page's rows at a time, into a ring of 32 KB slots
+//   warps 18, 19     complete the warpgroup that gives its registers away
 // Tensor memory (512 columns): S0, S1 (128 each; P overwrites the first half of its S), O0, O1.  MMAs execute in the order
 // of their issue, so S of the next tile may be issued behind the product that still reads P.  The running maximum moves
 // only when a row passes it by 2^8; then the row's thread rescales its accumulator in tensor memory, which nothing else
 // touches at that point: the product before has completed (the commit that announced S covers it), the next one waits
-// for P.
+// for P.  The second half of a row writes its P over scores of the first half, behind the vote, when those are read.
 #pragma once
 
 #include "paged_attn.cuh"
 
 namespace fa {
 
-constexpr int PT_THREADS = 384;                          // 168 registers each at launch, moved to where they are needed:
-constexpr int PT_SOFTMAX_REGS = 216, PT_OTHER_REGS = 72;   // 256 x 216 + 128 x 72 = 384 x 168
+constexpr int PT_THREADS = 640;                           // 96 registers each at launch, moved to where they are needed:
+constexpr int PT_SOFTMAX_REGS = 104, PT_OTHER_REGS = 64;   // 512 x 104 + 128 x 64 = 640 x 96
 constexpr int PT_ROWS = 256;
+
+// what a softmax warpgroup works on next, and where its walk stands: kept in shared memory by the warpgroup's first
+// thread, so that the walk takes no registers from the 128 scores of every thread
+struct PtSegment {
+  int more, row0, t0, n, L, h, t, t_end, first, last;   // more = 0: done
+};
+struct PtWalk {
+  PaUnit u;
+  PaRange r;
+  long long done;
+  int t;
+};
 
 template <int D>
 struct PaTile {
@@ -34,11 +51,14 @@ struct PaTile {
     uint64_t full[ST], empty[ST], q_full[2], s_full[2], p_full[2], o_full[2], tail;
     uint32_t bad[16];          // keys of a tile that no page holds, by groups of 16; the fetches are < 16 tiles ahead
     PaLocate loc;
+    PtWalk walk[2];
+    PtSegment seg[2];
+    float half[2][2][128];     // what the two halves of a row tell each other
     uint32_t tmem;
     int dead;
   };
-  static constexpr int SMEM = QBYTES + ST * SLOT + 1024;
-  static_assert(sizeof(Small) <= 1024, "barriers");
+  static constexpr int SMEM = QBYTES + ST * SLOT + 3072;
+  static_assert(sizeof(Small) <= 3072, "barriers");
 };
 
 struct PaTileParams {
@@ -63,6 +83,12 @@ __device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc) : "memory");
 }
+// one lane of a converged warp; what it computes stays in uniform registers
+__device__ __forceinline__ bool pt_elect() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+  return r != 0;
+}
 __device__ __forceinline__ void pt_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
 }
@@ -85,6 +111,49 @@ __device__ __forceinline__ void pt_st32(uint32_t taddr, const uint32_t* r) {
       "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
       "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(taddr),
       PT_W8(r, 0), PT_W8(r, 8), PT_W8(r, 16), PT_W8(r, 24) : "memory");
+}
+__device__ __forceinline__ void pt_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+      : PT_R8(r, 0), PT_R8(r, 8) : "r"(taddr));
+}
+__device__ __forceinline__ void pt_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(taddr),
+      PT_W8(r, 0), PT_W8(r, 8) : "memory");
+}
+// two float32 at a time
+__device__ __forceinline__ uint64_t pt_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void pt_unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t pt_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t pt_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// barrier of the 256 threads of a query tile, and the same with a vote
+__device__ __forceinline__ void pt_sync(int id) { asm volatile("bar.sync %0, 256;\n" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool pt_sync_any(int id, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbar.red.or.pred q, %1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(r) : "r"(id), "r"((uint32_t)x) : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ float pt_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 __device__ __forceinline__ void pt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
@@ -117,15 +186,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
       pa_bar_init(pa_smem(&sh.empty[s]), 1);
     }
     for (int w = 0; w < 2; ++w) {
-      pa_bar_init(pa_smem(&sh.q_full[w]), 128);
+      pa_bar_init(pa_smem(&sh.q_full[w]), 8);           // an arrival per warp: one per thread took as long as the exponentials
       pa_bar_init(pa_smem(&sh.s_full[w]), 1);
-      pa_bar_init(pa_smem(&sh.p_full[w]), 128);
+      pa_bar_init(pa_smem(&sh.p_full[w]), 8);
       pa_bar_init(pa_smem(&sh.o_full[w]), 1);
     }
     pa_bar_init(pa_smem(&sh.tail), 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(pa_smem(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
@@ -137,115 +206,147 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
   const uint32_t tmem = sh.tmem;
   long long done = range.beg;
 
-  if (warp < 8) {
+  if (warp < 16) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(PT_SOFTMAX_REGS));
     // ---- softmax ------------------------------------------------------------------------------------------------------
-    const int w = warp >> 2, i = tid & 127;
+    const int w = warp >> 3, half = (warp >> 2) & 1, i = tid & 127;   // query tile, half of the keys, row
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + w * 128 + lanes, to = tmem + 256 + w * 128 + lanes;
     const uint32_t s_full = pa_smem(&sh.s_full[w]), p_full = pa_smem(&sh.p_full[w]);
+    const float scale = c.scale_log2;
+    PtWalk& walk = sh.walk[w];
+    PtSegment& seg = sh.seg[w];
+    if (i == 0 && half == 0) walk.u = u, walk.r = range, walk.done = range.beg, walk.t = t;
     uint32_t s_par = 0, o_par = 0;
     int tile_no = 0;                                      // tiles since the start
-    while (done < range.end) {
-      if (t >= u.tiles) {
-        u.next(c, p);
-        t = 0;
-        continue;
+    for (;;) {
+      if (i == 0 && half == 0) {
+        seg.more = walk.done < walk.r.end;
+        if (seg.more) {
+          while (walk.t >= walk.u.tiles) walk.u.next(c, p), walk.t = 0;
+          const PaUnit& x = walk.u;
+          seg.t = walk.t;
+          seg.t_end = (int)min((long long)x.tiles, walk.t + (walk.r.end - walk.done));
+          seg.row0 = x.rb * PT_ROWS + w * 128;
+          seg.t0 = x.s.t0, seg.n = x.s.n, seg.L = x.s.L, seg.h = x.h;
+          seg.first = seg.t == 0, seg.last = seg.t_end == x.tiles;
+          if (seg.last && w == 0)
+            p.info[pa_unit_id(c, p, x.b, x.s, x.h, x.rb)] = make_int2(pa_owner(walk.r, walk.done - walk.t), blockIdx.x);
+          walk.done += seg.t_end - seg.t;
+          walk.t = seg.t_end;
+        }
       }
-      const int t_end = (int)min((long long)u.tiles, t + (range.end - done));
-      const int row0 = u.rb * PT_ROWS + w * 128;
-      const long long all_rows = (long long)u.s.n * c.G;
-      const int n_rows = (int)max(0LL, min(128LL, all_rows - row0));
+      pt_sync(1 + w);
+      if (!seg.more) break;
+      const int t_beg = seg.t, t_end = seg.t_end, row0 = seg.row0;
+      const int n_rows = (int)max(0LL, min(128LL, (long long)seg.n * c.G - row0));
       if (n_rows == 0) {
-        tile_no += t_end - t;
+        tile_no += t_end - t_beg;
       } else {
         // the query tile, zeros behind the last row
         const uint32_t qb = q_smem + w * C::SLOT;
+        {
+          const T* q = reinterpret_cast<const T*>(c.q) + (int64_t)seg.t0 * c.q_st + (int64_t)seg.h * c.G * c.q_sh;
 #pragma unroll 4
-        for (int e = i; e < 128 * (D / 8); e += 128) {
-          const int r = e / (D / 8), ch = e % (D / 8);
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (r < n_rows) {
-            const int tok = (row0 + r) / c.G, hg = (row0 + r) - tok * c.G;
-            v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(c.q) + (int64_t)(u.s.t0 + tok) * c.q_st +
-                                                (int64_t)(u.h * c.G + hg) * c.q_sh + ch * 8);
+          for (int e = half * 128 + i; e < 128 * (D / 8); e += 256) {
+            const int r = e / (D / 8), ch = e % (D / 8);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < n_rows) {
+              const int tok = (row0 + r) / c.G, hg = (row0 + r) - tok * c.G;
+              v = *reinterpret_cast<const uint4*>(q + (int64_t)tok * c.q_st + (int64_t)hg * c.q_sh + ch * 8);
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(qb + (ch >> 3) * C::HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
+                         "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
           }
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(qb + (ch >> 3) * C::HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
-                       "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
         }
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // generic writes -> MMA reads
         pt_before();
-        pa_bar_arrive(pa_smem(&sh.q_full[w]));
+        __syncwarp();
+        if (lane == 0) pa_bar_arrive(pa_smem(&sh.q_full[w]));
 
-        const int my_tok = (int)min((long long)row0 + i, all_rows - 1);
-        const int lim = p.prefix_len > 0 ? u.s.L : min(u.s.L, u.s.L - u.s.n + my_tok / c.G + 1);
+        const int lim = p.prefix_len > 0 ? seg.L : min(seg.L, seg.L - seg.n + (row0 + min(i, n_rows - 1)) / c.G + 1);
+        int nv = lim - t_beg * PA_TILE - 64 * half;       // keys of this half of the tile that the row sees
         float m = -INFINITY, l = 0.f;
-        for (int tt = t; tt < t_end; ++tt) {
+#pragma unroll 1
+        for (int left = t_end - t_beg; left > 0; --left, nv -= PA_TILE) {
           pa_bar_wait(s_full, s_par, dead);
           s_par ^= 1;
           pt_after();
-          uint32_t sr[128];
-          pt_ld32(ts, sr);
-          pt_ld32(ts + 32, sr + 32);
-          pt_ld32(ts + 64, sr + 64);
-          pt_ld32(ts + 96, sr + 96);
+          uint32_t sr[64];
+          pt_ld32(ts + 64 * half, sr);
+          pt_ld32(ts + 64 * half + 32, sr + 32);
           pt_wait_ld();
-          float* s = reinterpret_cast<float*>(sr);
-          const uint32_t bad = sh.bad[tile_no++ & 15];
-          const int nv = lim - tt * PA_TILE;              // keys of the tile this row sees
-          if (__any_sync(0xffffffffu, nv < PA_TILE || bad != 0)) {
+          const uint32_t bad = sh.bad[tile_no++ & 15] >> (4 * half);
+          if (__any_sync(0xffffffffu, nv < 64 || bad != 0)) {
 #pragma unroll
-            for (int j = 0; j < 128; ++j)
-              if (j >= nv || ((bad >> (j / 16)) & 1)) s[j] = -INFINITY;
+            for (int j = 0; j < 64; ++j)
+              if (j >= nv || ((bad >> (j / 16)) & 1)) sr[j] = 0xff800000u;
           }
-          float mx[4] = {s[0], s[1], s[2], s[3]};
+          float mx[4];
 #pragma unroll
-          for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c.scale_log2;
-          if (__any_sync(0xffffffffu, top > m + 8.f)) {
-            const float nm = fmaxf(m, top);
+          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(__uint_as_float(sr[k]), __uint_as_float(sr[4 + k]));
+#pragma unroll
+          for (int j = 8; j < 64; j += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mx[k] = pt_max3(mx[k], __uint_as_float(sr[j + k]), __uint_as_float(sr[j + 4 + k]));
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+          if (pt_sync_any(1 + w, top > m + 8.f)) {
+            sh.half[w][half][i] = top;
+            pt_sync(1 + w);
+            const float nm = fmaxf(m, fmaxf(top, sh.half[w][half ^ 1][i]));
             const float f = m == -INFINITY ? 0.f : pa_ex2(m - nm);
             m = nm;
             l *= f;
-            if (tt > t) {
-#pragma unroll
-              for (int j = 0; j < D; j += 32) {
-                uint32_t o[32];
-                pt_ld32(to + j, o);
+            if (left < t_end - t_beg) {
+#pragma unroll 1
+              for (int j = half * (D / 2); j < (half + 1) * (D / 2); j += 16) {
+                uint32_t o[16];
+                pt_ld16(to + j, o);
                 pt_wait_ld();
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                pt_st32(to + j, o);
+                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                pt_st16(to + j, o);
               }
             }
+            pt_sync(1 + w);                               // sh.half has been read
           }
-          const float off = m == -INFINITY ? 0.f : m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const float off = m == -INFINITY ? 0.f : -m;
+          const uint64_t sc2 = pt_pair(scale, scale), off2 = pt_pair(off, off);
+          uint64_t sum[2] = {0, 0};
 #pragma unroll
-          for (int j = 0; j < 128; ++j) {
-            s[j] = pa_ex2(fmaf(s[j], c.scale_log2, -off));
-            sum[j & 3] += s[j];
+          for (int j = 0; j < 32; ++j) {
+            float a, b;
+            pt_unpair(pt_fma2(pt_pair(__uint_as_float(sr[2 * j]), __uint_as_float(sr[2 * j + 1])), sc2, off2), a, b);
+            a = pa_ex2(a), b = pa_ex2(b);
+            sum[j & 1] = pt_add2(sum[j & 1], pt_pair(a, b));
+            sr[j] = pa_pack<T>(a, b);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-          for (int j = 0; j < 64; ++j) sr[j] = pa_pack<T>(s[2 * j], s[2 * j + 1]);
-          pt_st32(ts, sr);
-          pt_st32(ts + 32, sr + 32);
+          pt_st32(ts + 32 * half, sr);
+          {
+            float a, b;
+            pt_unpair(pt_add2(sum[0], sum[1]), a, b);
+            l += a + b;
+          }
           pt_wait_st();
           pt_before();
-          pa_bar_arrive(p_full);
+          __syncwarp();
+          if (lane == 0) pa_bar_arrive(p_full);
         }
         // ---- this segment's result ------------------------------------------------------------------------------------
         pa_bar_wait(pa_smem(&sh.o_full[w]), o_par, dead);
         o_par ^= 1;
         pt_after();
-        const bool first = t == 0, last = t_end == u.tiles, whole = first && last;
+        const bool whole = seg.first && seg.last;
+        sh.half[w][half][i] = l;
+        pt_sync(1 + w);
+        l += sh.half[w][half ^ 1][i];
         if (*dead) l = __int_as_float(0x7fc00000);
         const int r = row0 + i;
-        const int tok = u.s.t0 + r / c.G, hq = u.h * c.G + r % c.G;
+        const int tok = seg.t0 + r / c.G, hq = seg.h * c.G + r % c.G;
+        const int64_t at = whole ? (int64_t)tok * c.Hq + hq : (int64_t)(2 * blockIdx.x + (seg.first ? 1 : 0)) * PT_ROWS + w * 128 + i;
         const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-        for (int j = 0; j < D; j += 32) {
+#pragma unroll 1
+        for (int j = half * (D / 2); j < (half + 1) * (D / 2); j += 32) {
           uint32_t o[32];
           pt_ld32(to + j, o);
           pt_wait_ld();
@@ -258,37 +359,49 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
 #pragma unroll
             for (int k = 0; k < 4; ++k) dst[k] = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
           } else {
-            const int64_t at = whole ? (int64_t)tok * c.Hq + hq : (int64_t)(2 * blockIdx.x + (first ? 1 : 0)) * PT_ROWS + w * 128 + i;
             uint4* dst = reinterpret_cast<uint4*>((whole ? p.row_o : p.slot_o) + at * D + j);
 #pragma unroll
             for (int k = 0; k < 8; ++k) dst[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
         }
-        if (i < n_rows) {
+        if (i < n_rows && half == 0) {
           if (whole && p.direct) {
             if (c.lse) c.lse[(int64_t)tok * c.Hq + hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
           } else {
-            const int64_t at = whole ? (int64_t)tok * c.Hq + hq : (int64_t)(2 * blockIdx.x + (first ? 1 : 0)) * PT_ROWS + w * 128 + i;
             (whole ? p.row_ml : p.slot_ml)[at] = make_float2(m, l);
           }
         }
         pt_before();
-        if (last && w == 0 && i == 0)
-          p.info[pa_unit_id(c, p, u.b, u.s, u.h, u.rb)] = make_int2(pa_owner(range, done - t), blockIdx.x);
       }
-      done += t_end - t;
-      t = t_end;
+      pt_sync(1 + w);   // everyone has read the segment
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PT_OTHER_REGS));
   }
-  if (warp == 8) {
+  if (warp == 16) {
     // ---- the MMAs -----------------------------------------------------------------------------------------------------
     constexpr uint32_t F = PtFormat<T>::F;
-    const uint32_t id_qk = (1u << 4) | (F << 7) | (F << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-    const uint32_t id_pv = (1u << 4) | (F << 7) | (F << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t id_qk = (1u << 4) | (F << 7) | (F << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t id_pv = (1u << 4) | (F << 7) | (F << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
+    const uint64_t q_desc = pt_desc(q_smem, 16, 1024), k_desc = pt_desc(ring, 16, 1024), v_desc = pt_desc(ring, C::HALF, 1024);
     int slot = 0;
     uint32_t par = 0, q_par = 0, p_par = 0;               // q_par, p_par: a bit per query tile
+    auto advance = [&]() {
+      if (++slot == C::ST) slot = 0, par ^= 1;
+    };
+    auto scores = [&](int w, int k_slot) {
+      if (pt_elect()) {
+        const uint64_t qd = q_desc + w * (C::SLOT >> 4), kd = k_desc + k_slot * (C::SLOT >> 4);
+        const uint32_t s_tm = tmem + w * 128;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t o = ((kk >> 2) * C::HALF + (kk & 3) * 32) >> 4;
+          pt_mma_ss(s_tm, qd + o, kd + o, id_qk, kk > 0);
+        }
+        pt_commit(pa_smem(&sh.s_full[w]));
+      }
+      __syncwarp();
+    };
     while (done < range.end) {
       if (t >= u.tiles) {
         u.next(c, p);
@@ -297,58 +410,50 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
       }
       const int t_end = (int)min((long long)u.tiles, t + (range.end - done));
       const int nw = (long long)u.s.n * c.G - (long long)u.rb * PT_ROWS > 128 ? 2 : 1;
-      auto scores = [&](int w, uint32_t kb) {
-        if (lane == 0) {
-          const uint32_t qb = q_smem + w * C::SLOT;
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t o = (kk >> 2) * C::HALF + (kk & 3) * 32;
-            pt_mma_ss(tmem + w * 128, pt_desc(qb + o, 16, 1024), pt_desc(kb + o, 16, 1024), id_qk, kk > 0);
-          }
-          pt_commit(pa_smem(&sh.s_full[w]));
-        }
-        __syncwarp();
-      };
-      auto advance = [&]() {
-        if (++slot == C::ST) slot = 0, par ^= 1;
-      };
       // K of the first tile
       pa_bar_wait(pa_smem(&sh.full[slot]), par, dead);
       for (int w = 0; w < nw; ++w) {
         pa_bar_wait(pa_smem(&sh.q_full[w]), (q_par >> w) & 1, dead);
         q_par ^= 1u << w;
         pt_after();
-        scores(w, ring + slot * C::SLOT);
+        scores(w, slot);
       }
-      if (lane == 0) pt_commit(pa_smem(&sh.empty[slot]));
+      if (pt_elect()) pt_commit(pa_smem(&sh.empty[slot]));
       __syncwarp();
       advance();
       for (int tt = t; tt < t_end; ++tt) {
         const bool more = tt + 1 < t_end;
-        const int nv = min(PA_TILE, u.limit - tt * PA_TILE), steps = (nv + 15) / 16;
+        const int steps = (min(PA_TILE, u.limit - tt * PA_TILE) + 15) / 16;
         const int v_slot = slot;
-        const uint32_t vb = ring + slot * C::SLOT;
         pa_bar_wait(pa_smem(&sh.full[slot]), par, dead);
         advance();
         const int k_slot = slot;
-        if (more) {
-          pa_bar_wait(pa_smem(&sh.full[slot]), par, dead);
-          advance();
-        }
+        const uint32_t k_par = par;
+        if (more) advance();
         for (int w = 0; w < nw; ++w) {
           pa_bar_wait(pa_smem(&sh.p_full[w]), (p_par >> w) & 1, dead);
           p_par ^= 1u << w;
           pt_after();
-          if (lane == 0) {
-            for (int kk = 0; kk < steps; ++kk)
-              pt_mma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8, pt_desc(vb + kk * 2048, C::HALF, 1024), id_pv,
-                        tt > t || kk > 0);
+          if (pt_elect()) {
+            const uint64_t vd = v_desc + v_slot * (C::SLOT >> 4);
+            const uint32_t p_tm = tmem + w * 128, o_tm = tmem + 256 + w * 128;
+            if (steps == PA_TILE / 16) {
+#pragma unroll
+              for (int kk = 0; kk < PA_TILE / 16; ++kk)
+                pt_mma_ts(o_tm, p_tm + kk * 8, vd + kk * (2048 >> 4), id_pv, kk > 0 || tt > t);
+            } else {
+              for (int kk = 0; kk < steps; ++kk)
+                pt_mma_ts(o_tm, p_tm + kk * 8, vd + kk * (2048 >> 4), id_pv, kk > 0 || tt > t);
+            }
             if (!more) pt_commit(pa_smem(&sh.o_full[w]));
           }
           __syncwarp();
-          if (more) scores(w, ring + k_slot * C::SLOT);
+          if (more) {
+            if (w == 0) pa_bar_wait(pa_smem(&sh.full[k_slot]), k_par, dead);
+            scores(w, k_slot);
+          }
         }
-        if (lane == 0) {
+        if (pt_elect()) {
           pt_commit(pa_smem(&sh.empty[v_slot]));
           if (more) pt_commit(pa_smem(&sh.empty[k_slot]));
         }
@@ -357,36 +462,38 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
       done += t_end - t;
       t = t_end;
     }
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     // ---- the fetches --------------------------------------------------------------------------------------------------
     int slot = 0, tile_no = 0;
     uint32_t par = 1, t_par = 0;                          // the first pass over the ring finds it empty
-    const int n_box = PA_TILE / prm.box_rows;
-    const uint32_t box_bytes = prm.box_rows * 128;
+    const int box_keys = prm.box_rows;
+    const uint32_t box_bytes = box_keys * 128;
+    // lane i holds the page id of box i of the tile to come, requested while the tile before is fetched
+    auto page_id = [&]() -> int {
+      const int key = t * PA_TILE + lane * box_keys;
+      return lane * box_keys < PA_TILE && key < u.limit ? p.table[(int64_t)u.b * p.table_sb + key / c.page_size] : 0;
+    };
+    auto to_tile = [&]() {
+      while (done < range.end && t >= u.tiles) u.next(c, p), t = 0;
+    };
+    to_tile();
+    int next_id = done < range.end ? page_id() : 0;
     while (done < range.end) {
-      if (t >= u.tiles) {
-        u.next(c, p);
-        t = 0;
-        continue;
-      }
       const int key0 = t * PA_TILE, nv = min(PA_TILE, u.limit - key0);
-      const int need = (nv + prm.box_rows - 1) / prm.box_rows;        // boxes with keys
-      int page = c.num_pages, row = 0;
-      bool ok = true;
-      if (lane < need) {
-        const int key = key0 + lane * prm.box_rows;
-        page = p.table[(int64_t)u.b * p.table_sb + key / c.page_size];
-        row = key % c.page_size;
-        ok = page >= 0 && page < c.num_pages;
-        if (!ok) page = c.num_pages;                      // out of the map's range: zeros arrive
-      }
+      const int need = (nv + box_keys - 1) / box_keys;                // boxes with keys
+      const int row = (key0 + lane * box_keys) % c.page_size, head = u.h, L = u.s.L;
+      int page = next_id;
+      const bool ok = lane >= need || (page >= 0 && page < c.num_pages);
+      if (!ok) page = c.num_pages;                        // out of the map's range: zeros arrive
       // groups of 16 keys whose page id names no page
       const uint32_t miss = __ballot_sync(0xffffffffu, !ok);
       uint32_t bad = 0;
-      for (int b = 0; b < n_box; ++b)
-        if ((miss >> b) & 1)
-          for (int g = b * (prm.box_rows / 16); g < (b + 1) * (prm.box_rows / 16); ++g) bad |= 1u << g;
-      const bool tail = key0 + PA_TILE > u.s.L && (u.s.L & 15);        // keys and leftovers in one group of 16
+      if (miss != 0)
+        for (int g = 0; g < PA_TILE / 16; ++g) bad |= ((miss >> (g * 16 / box_keys)) & 1u) << g;
+      const bool tail = key0 + PA_TILE > L && (L & 15);               // keys and leftovers in one group of 16
+      ++done, ++t;
+      to_tile();
+      if (done < range.end) next_id = page_id();
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
         const uint32_t dst = ring + slot * C::SLOT, full = pa_smem(&sh.full[slot]);
@@ -399,13 +506,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         __syncwarp();
         if (lane < need)
           for (int hf = 0; hf < D / 64; ++hf)
-            pa_tma(dst + hf * C::HALF + lane * box_bytes, kv == 0 ? &prm.tm_k : &prm.tm_v, 64 * hf, row, u.h, page, bar);
+            pa_tma(dst + hf * C::HALF + lane * box_bytes, kv == 0 ? &prm.tm_k : &prm.tm_v, 64 * hf, row, head, page, bar);
         if (kv == 1 && tail) {
           // rows behind the sequence hold anything, and 0 x NaN must not reach the sums: zeros up to the end of the
           // group of 16 (the product stops there)
           pa_bar_wait(bar, t_par, dead);
           t_par ^= 1;
-          const int r0 = u.s.L - key0, r1 = (r0 + 15) & ~15;
+          const int r0 = L - key0, r1 = (r0 + 15) & ~15;
           for (int e = lane; e < (r1 - r0) * (D / 8); e += 32) {
             const int r = r0 + e / (D / 8), ch = e % (D / 8);
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(dst + (ch >> 3) * C::HALF + r * 128 + ((ch & 7) << 4)), "r"(0) : "memory");
@@ -416,7 +523,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         }
         if (++slot == C::ST) slot = 0, par ^= 1;
       }
-      ++done, ++t, ++tile_no;
+      ++tile_no;
     }
   }
   if (*dead) {
@@ -426,7 +533,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
   }
   pt_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     pt_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
   }
