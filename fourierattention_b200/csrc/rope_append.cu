@@ -5,11 +5,12 @@
 //   z[d]       = y[d],  d >= R;      a_i = position * inv_freq[i]
 // All arithmetic in float32, one rounding at the store.
 //
-// Bound: HBM (every element is read and written once, ~10 flop each).  A CTA takes TOK tokens; their angles are
-// reduced in float64 (a float32 product is off by 0.008 rad at position 131072), once per token, and shared by all of
-// its heads through shared memory.  D/16 neighbouring lanes hold a head, 8 + 8 elements each (the two halves of eight
-// rotation pairs), so that the mean square is a few shuffles and every access is 16 bytes.  Each thread requests its
-// first elements before it computes angles.
+// Bound: HBM (every element is read and written once, ~10 flop each), and close behind it the issue of instructions.
+// A warp takes a token (of few tokens: some of its heads; of many, one token after another) and walks its heads, D/16 neighbouring lanes to a head, each
+// with 8 + 8 elements: the two halves of eight rotation pairs.  So the mean square is a few shuffles, every access is
+// 16 bytes, cosines, sines and weights stay in registers for all heads, and the arithmetic runs on pairs of floats
+// (f32x2).  The next heads are requested across the token's end.  Angles are reduced in float64 (a float32 product is off by 0.008 rad at position 131072), once per warp
+// and token, two pairs to a lane.
 #include "common.cuh"
 
 namespace fa {
@@ -17,212 +18,231 @@ namespace fa {
 struct RopeParams {
   fa_rope_args_t a;
   int lph_log2;   // lanes per head, log2
-  int append;
+  int chunks;     // warps per token
+  int warps;      // of the grid
 };
 
-constexpr int RA_THREADS = 256;
-constexpr int RA_MAX_TOK = 4;
+constexpr int RA_WARPS = 8;
 constexpr int RA_MAX_PAIRS = 128;
-constexpr int RA_BATCH = 4;   // heads in flight per thread
+constexpr int RA_AHEAD = 3;   // heads in flight per lane
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void ra_load(const T* p, float* f) {
-  if (VEC) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(p);
-    unpack8<T>(raw, f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f32(p[i]);
-  }
-}
-__device__ __forceinline__ void ra_cvt(float f, __half* o) { *o = __float2half_rn(f); }
-__device__ __forceinline__ void ra_cvt(float f, __nv_bfloat16* o) { *o = __float2bfloat16_rn(f); }
-template <typename T, bool VEC>
-__device__ __forceinline__ void ra_store(T* p, const float* f) {
+__device__ __forceinline__ uint4 ra_load(const T* p) {
+  if (VEC) return *reinterpret_cast<const uint4*>(p);
   alignas(16) T v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ra_cvt(f[i], v + i);
+  for (int i = 0; i < 8; ++i) v[i] = p[i];
+  return *reinterpret_cast<const uint4*>(v);
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void ra_store(T* p, const uint4& raw) {
   if (VEC) {
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
+    *reinterpret_cast<uint4*>(p) = raw;
   } else {
+    const T* v = reinterpret_cast<const T*>(&raw);
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = v[i];
   }
 }
+// pairs of floats
+__device__ __forceinline__ uint64_t ra_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 ra_split(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t ra_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t ra_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 template <typename T>
-__device__ __forceinline__ void ra_weight(const void* w, int f32, int d, float* f) {
+__device__ __forceinline__ void ra_unpack(const uint4& raw, uint64_t* x) {
+  const typename Pack2<T>::type* p = reinterpret_cast<const typename Pack2<T>::type*>(&raw);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = f32 ? reinterpret_cast<const float*>(w)[d + i] : to_f32(reinterpret_cast<const T*>(w)[d + i]);
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = Pack2<T>::cvt(p[i]);
+    x[i] = ra_pair(v.x, v.y);
+  }
+}
+__device__ __forceinline__ uint32_t ra_round(uint64_t v, __half) {
+  const float2 f = ra_split(v);
+  const __half2 h = __floats2half2_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t ra_round(uint64_t v, __nv_bfloat16) {
+  const float2 f = ra_split(v);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <typename T, int TOK, bool VEC>
-__global__ void __launch_bounds__(RA_THREADS) rope_kernel(const __grid_constant__ RopeParams prm) {
+template <typename T, bool VEC, bool APPEND>
+__global__ void __launch_bounds__(RA_WARPS * 32, 2) rope_kernel(const __grid_constant__ RopeParams prm) {
   const fa_rope_args_t& a = prm.a;
-  __shared__ float s_cos[TOK][RA_MAX_PAIRS], s_sin[TOK][RA_MAX_PAIRS];
-  __shared__ long long s_pos[TOK];     // position of the token
-  __shared__ int s_live[TOK];          // the token belongs to a sequence
-  __shared__ long long s_kdst[TOK], s_vdst[TOK];   // element offset of (page, head 0, row) or -1: not stored
-  const int tid = threadIdx.x;
-  const int t0 = blockIdx.x * TOK;
-  const int lph = 1 << prm.lph_log2;
-  const int heads = a.Hq + a.Hkv + (prm.append ? a.Hkv : 0);
-  const int total = TOK * heads;                       // (token, head) pairs of this CTA
-  const int c = tid & (lph - 1);                       // chunk of the head this lane holds
-  const int first = tid >> prm.lph_log2, step = RA_THREADS >> prm.lph_log2;
+  __shared__ __align__(16) float s_cos[RA_WARPS][RA_MAX_PAIRS], s_sin[RA_WARPS][RA_MAX_PAIRS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int unit = blockIdx.x * RA_WARPS + warp;
+  int t = unit / prm.chunks;                               // the token at work
+  const int chunk = unit - t * prm.chunks, stride = prm.warps / prm.chunks;
+  const int heads = a.Hq + a.Hkv + (APPEND ? a.Hkv : 0);
+  const int per = 32 >> prm.lph_log2;                      // heads a warp holds at once
+  const int groups = (heads + per - 1) / per;
+  const int g0 = groups * chunk / prm.chunks, g1 = groups * (chunk + 1) / prm.chunks;
+  const int c = lane & ((1 << prm.lph_log2) - 1);          // chunk of the head this lane holds
   const bool lane_on = c * 16 < a.D;
   const int nrot = a.R / 16;
-  // element offsets of the two halves of the chunk: a rotation pair, or 16 elements behind the rotary width
+  // the two halves of the chunk: a rotation pair, or 16 elements behind the rotary width
   const int lo = c < nrot ? 8 * c : a.R + 16 * (c - nrot);
   const int hi = c < nrot ? a.R / 2 + 8 * c : lo + 8;
+  const int sub = lane >> prm.lph_log2;                    // which of the heads held at once
+  const int h_end = min(heads, g1 * per);
 
-  auto source = [&](int it, int& kind, int& tok, int& h) -> const T* {
-    tok = it / heads;
-    const int x = it - tok * heads;
-    const int64_t t = t0 + tok;
-    if (x < a.Hq) {
-      kind = 0, h = x;
-      return reinterpret_cast<const T*>(a.q) + t * a.q_st + (int64_t)h * a.q_sh;
+  uint4 raw[RA_AHEAD][2];
+  int rt = t, rg = g0;                                     // token and heads of the next request
+  auto request = [&](uint4* r) {
+    r[0] = r[1] = make_uint4(0, 0, 0, 0);
+    const int head = rg * per + sub;
+    if (lane_on && head < h_end && rt < a.tokens) {
+      const T* p;
+      if (head < a.Hq) p = reinterpret_cast<const T*>(a.q) + (int64_t)rt * a.q_st + (int64_t)head * a.q_sh;
+      else if (head < a.Hq + a.Hkv) p = reinterpret_cast<const T*>(a.k) + (int64_t)rt * a.k_st + (int64_t)(head - a.Hq) * a.k_sh;
+      else p = reinterpret_cast<const T*>(a.v) + (int64_t)rt * a.v_st + (int64_t)(head - a.Hq - a.Hkv) * a.v_sh;
+      r[0] = ra_load<T, VEC>(p + lo);
+      r[1] = ra_load<T, VEC>(p + hi);
     }
-    if (x < a.Hq + a.Hkv) {
-      kind = 1, h = x - a.Hq;
-      return reinterpret_cast<const T*>(a.k) + t * a.k_st + (int64_t)h * a.k_sh;
-    }
-    kind = 2, h = x - a.Hq - a.Hkv;
-    return reinterpret_cast<const T*>(a.v) + t * a.v_st + (int64_t)h * a.v_sh;
+    if (++rg == g1) rg = g0, rt += stride;
   };
-
-  // ---- request the first batch of elements ---------------------------------------------------------------------
-  float x[RA_BATCH][16];
-  auto load_batch = [&](int base) {
 #pragma unroll
-    for (int u = 0; u < RA_BATCH; ++u) {
-      const int it = base + u * step;
-      int kind, tok, h;
-      if (it < total && lane_on && t0 + it / heads < a.tokens) {
-        const T* p = source(it, kind, tok, h);
-        ra_load<T, VEC>(p + lo, x[u]);
-        ra_load<T, VEC>(p + hi, x[u] + 8);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
-      }
-    }
-  };
-  load_batch(first);
+  for (int u = 0; u < RA_AHEAD; ++u) request(raw[u]);
 
-  // ---- where the tokens belong ---------------------------------------------------------------------------------
-  int seq0 = 0;
-  if (prm.append && a.cu_seqlens) {
-    // sequences that end at or before token t0; rows of empty sequences are passed over
-    int n = 0;
-    for (int b = tid; b < a.B; b += RA_THREADS) n += a.cu_seqlens[b + 1] <= t0;
-    __shared__ int s_n[RA_THREADS / 32];
-    n = __reduce_add_sync(0xffffffffu, n);
-    if ((tid & 31) == 0) s_n[tid >> 5] = n;
-    __syncthreads();
-    for (int w = 0; w < RA_THREADS / 32; ++w) seq0 += s_n[w];
-  }
-  if (tid < TOK) {
-    const int t = t0 + tid;
-    bool live = t < a.tokens;
-    long long pos = 0, kdst = -1, vdst = -1;
-    if (prm.append && live) {
-      int b, i, n;
+  bool live = true;                                        // the token belongs to a sequence
+  long long kdst = -1, vdst = -1;                          // element offset of (page, head 0, row); -1: not stored
+  uint64_t cs[4], sn[4];                                   // elements behind the rotary width turn by nothing
+  auto begin_token = [&]() {
+    // ---- where the token belongs ---------------------------------------------------------------------------------
+    long long pos = 0;
+    if (APPEND) {
+      int b = t, i = 0, n = 1;
+      kdst = vdst = -1;
       if (a.cu_seqlens) {
-        b = seq0;
-        while (b < a.B && a.cu_seqlens[b + 1] <= t) ++b;
-        live = b < a.B;
-        if (live) {
+        // sequences that end at or before the token; empty ones are passed over
+        int before = 0;
+        for (int x = lane; x < a.B; x += 32) before += a.cu_seqlens[x + 1] <= t;
+        b = __reduce_add_sync(0xffffffffu, before);
+        if (b < a.B) {
           const int beg = a.cu_seqlens[b];
           i = t - beg;
           n = a.cu_seqlens[b + 1] - beg;
         }
-      } else {
-        b = t, i = 0, n = 1;
-        live = b < a.B;
       }
-      if (live) {
-        const long long j = (long long)a.kv_lens[b] - n + i;   // index in its own sequence
-        pos = a.pos_offset + j;
-        const long long pg = j >= 0 ? j / a.page_size : -1;
-        if (i >= 0 && pg >= 0 && pg < a.max_pages) {
-          const int page = a.page_table[(int64_t)b * a.table_sb + pg];
-          if (page >= 0 && page < a.num_pages) {
-            const long long row = j - pg * a.page_size;
-            kdst = (long long)page * a.kp_sp + row * a.kp_sr;
-            vdst = (long long)page * a.vp_sp + row * a.vp_sr;
-          }
+      live = b < a.B;
+      if (!live) return;                                   // behind the last sequence: left as it was
+      const long long j = (long long)a.kv_lens[b] - n + i; // index in its own sequence
+      pos = a.pos_offset + j;
+      const long long pg = j >= 0 ? j / a.page_size : -1;
+      if (i >= 0 && pg >= 0 && pg < a.max_pages) {
+        const int page = a.page_table[(int64_t)b * a.table_sb + pg];
+        if (page >= 0 && page < a.num_pages) {
+          const long long row = j - pg * a.page_size;
+          kdst = (long long)page * a.kp_sp + row * a.kp_sr;
+          vdst = (long long)page * a.vp_sp + row * a.vp_sr;
         }
       }
     }
-    if (live && a.positions)
+    if (a.positions)
       pos = a.pos_i64 ? reinterpret_cast<const long long*>(a.positions)[t] : (long long)reinterpret_cast<const int*>(a.positions)[t];
-    s_pos[tid] = pos;
-    s_live[tid] = live;
-    s_kdst[tid] = kdst;
-    s_vdst[tid] = vdst;
-  }
-  __syncthreads();
-  // ---- angles: turns in float64, the fraction of a turn in float32 -----------------------------------------------
-  for (int i = tid; i < TOK * (a.R / 2); i += RA_THREADS) {
-    const int tok = i / (a.R / 2), p = i - tok * (a.R / 2);
-    double turns = (double)s_pos[tok] * (double)a.inv_freq[p] * 0.15915494309189533577;   // 1 / (2 pi)
-    turns -= rint(turns);
-    float sn, cs;
-    sincospif(2.0f * (float)turns, &sn, &cs);
-    s_cos[tok][p] = cs;
-    s_sin[tok][p] = sn;
-  }
-  __syncthreads();
+    // ---- angles: turns in float64, the fraction of a turn in float32 -----------------------------------------------
+    __syncwarp();
+    for (int p = lane; p < a.R / 2; p += 32) {
+      double turns = (double)pos * (double)a.inv_freq[p] * 0.15915494309189533577;   // 1 / (2 pi)
+      turns -= rint(turns);
+      sincospif(2.0f * (float)turns, &s_sin[warp][p], &s_cos[warp][p]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      cs[i] = c < nrot ? *reinterpret_cast<const uint64_t*>(&s_cos[warp][8 * c + 2 * i]) : ra_pair(1.f, 1.f);
+      sn[i] = c < nrot ? *reinterpret_cast<const uint64_t*>(&s_sin[warp][8 * c + 2 * i]) : 0;
+    }
+  };
 
-  for (int base = first; base - first < total; base += RA_BATCH * step) {
-    if (base != first) load_batch(base);
+  uint64_t w[8];
+  int w_kind = -1;
+  const float inv_d = 1.0f / (float)a.D;
+  auto work = [&](int h, uint4* r) {
+    const int kind = h < a.Hq ? 0 : h < a.Hq + a.Hkv ? 1 : 2;
+    const void* wp = kind == 0 ? a.q_weight : kind == 1 ? a.k_weight : nullptr;
+    uint64_t x[8];
+    ra_unpack<T>(r[0], x);
+    ra_unpack<T>(r[1], x + 4);
+    float ss = 0.f;
+    if (a.q_weight || a.k_weight) {
+      // every lane takes part in the shuffles; heads without a weight drop the result
+      uint64_t acc = ra_mul(x[0], x[0]);
 #pragma unroll
-    for (int u = 0; u < RA_BATCH; ++u) {
-      const int it = base + u * step;
-      int kind = 2, tok = 0, h = 0;
-      if (it < total) source(it, kind, tok, h);
-      const bool on = it < total && lane_on && s_live[tok];
-      const void* w = kind == 0 ? a.q_weight : kind == 1 ? a.k_weight : nullptr;
-      // every lane of a warp takes part in the shuffles; heads without a weight drop the result
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) ss = fmaf(x[u][i], x[u][i], ss);
-      for (int o = lph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (!on) continue;
-      if (w) {
-        const float r = 1.0f / sqrtf(ss / (float)a.D + a.eps);
-        float wl[8], wh[8];
-        ra_weight<T>(w, a.w_f32, lo, wl);
-        ra_weight<T>(w, a.w_f32, hi, wh);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[u][i] *= r * wl[i];
-          x[u][8 + i] *= r * wh[i];
-        }
-      }
-      if (kind != 2 && c < nrot) {
+      for (int i = 1; i < 8; ++i) acc = ra_fma(x[i], x[i], acc);
+      const float2 f = ra_split(acc);
+      ss = f.x + f.y;
+      for (int o = (1 << prm.lph_log2) >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    }
+    if (!lane_on || h >= h_end || !live) return;
+    if (wp) {
+      if (w_kind != kind) {
+        w_kind = kind;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float cs = s_cos[tok][8 * c + i], sn = s_sin[tok][8 * c + i];
-          const float y0 = x[u][i], y1 = x[u][8 + i];
-          x[u][i] = y0 * cs - y1 * sn;
-          x[u][8 + i] = y1 * cs + y0 * sn;
+          const int d = (i < 4 ? lo : hi - 8) + 2 * i;
+          w[i] = a.w_f32 ? ra_pair(reinterpret_cast<const float*>(wp)[d], reinterpret_cast<const float*>(wp)[d + 1])
+                         : ra_pair(to_f32(reinterpret_cast<const T*>(wp)[d]), to_f32(reinterpret_cast<const T*>(wp)[d + 1]));
         }
       }
-      T* dst;
-      if (kind == 0) {
-        dst = reinterpret_cast<T*>(a.q_out) + (int64_t)(t0 + tok) * a.qo_st + (int64_t)h * a.qo_sh;
-      } else if (!prm.append) {
-        dst = reinterpret_cast<T*>(a.k_out) + (int64_t)(t0 + tok) * a.ko_st + (int64_t)h * a.ko_sh;
-      } else {
-        const long long at = kind == 1 ? s_kdst[tok] : s_vdst[tok];
-        if (at < 0) continue;
-        dst = kind == 1 ? reinterpret_cast<T*>(a.k_pages) + at + (int64_t)h * a.kp_sh
-                        : reinterpret_cast<T*>(a.v_pages) + at + (int64_t)h * a.vp_sh;
+      const float q = rsqrtf(fmaf(ss, inv_d, a.eps));
+      const uint64_t q2 = ra_pair(q, q);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = ra_mul(ra_mul(x[i], q2), w[i]);
+    }
+    if (kind != 2) {
+      uint32_t out[8];
+      const uint64_t minus = ra_pair(-1.f, -1.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        out[i] = ra_round(ra_fma(x[i], cs[i], ra_mul(ra_mul(x[4 + i], sn[i]), minus)), T());
+        out[4 + i] = ra_round(ra_fma(x[4 + i], cs[i], ra_mul(x[i], sn[i])), T());
       }
-      ra_store<T, VEC>(dst + lo, x[u]);
-      ra_store<T, VEC>(dst + hi, x[u] + 8);
+      r[0] = make_uint4(out[0], out[1], out[2], out[3]);
+      r[1] = make_uint4(out[4], out[5], out[6], out[7]);
+    }
+    T* dst;
+    if (kind == 0) {
+      dst = reinterpret_cast<T*>(a.q_out) + (int64_t)t * a.qo_st + (int64_t)h * a.qo_sh;
+    } else if (!APPEND) {
+      dst = reinterpret_cast<T*>(a.k_out) + (int64_t)t * a.ko_st + (int64_t)(h - a.Hq) * a.ko_sh;
+    } else {
+      if (kdst < 0) return;
+      dst = kind == 1 ? reinterpret_cast<T*>(a.k_pages) + kdst + (int64_t)(h - a.Hq) * a.kp_sh
+                      : reinterpret_cast<T*>(a.v_pages) + vdst + (int64_t)(h - a.Hq - a.Hkv) * a.vp_sh;
+    }
+    ra_store<T, VEC>(dst + lo, r[0]);
+    ra_store<T, VEC>(dst + hi, r[1]);
+  };
+  int g = g0;
+  while (t < a.tokens) {
+#pragma unroll
+    for (int u = 0; u < RA_AHEAD; ++u) {
+      if (t >= a.tokens) break;
+      if (g == g0) begin_token();
+      work(g * per + sub, raw[u]);
+      request(raw[u]);
+      if (++g == g1) g = g0, t += stride;
     }
   }
 }
@@ -231,22 +251,11 @@ static bool al16(const void* p, int64_t s0, int64_t s1) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s0 % 8 == 0 && s1 % 8 == 0;
 }
 
-template <typename T, int TOK, bool VEC>
-static void rope_launch(const RopeParams& prm, cudaStream_t st) {
-  rope_kernel<T, TOK, VEC><<<ceil_div(prm.a.tokens, TOK), RA_THREADS, 0, st>>>(prm);
-}
-template <typename T>
-static void rope_launch_t(const RopeParams& prm, bool vec, cudaStream_t st) {
-  // one token per CTA until every SM has several: a lone token's latency is the call's; from there on four tokens
-  // share the set-up
-  const bool many = prm.a.tokens >= 16 * sm_count();
-  if (many) {
-    if (vec) rope_launch<T, RA_MAX_TOK, true>(prm, st);
-    else rope_launch<T, RA_MAX_TOK, false>(prm, st);
-  } else {
-    if (vec) rope_launch<T, 1, true>(prm, st);
-    else rope_launch<T, 1, false>(prm, st);
-  }
+template <typename T, bool APPEND>
+static void rope_launch(const RopeParams& prm, bool vec, cudaStream_t st) {
+  const unsigned grid = prm.warps / RA_WARPS;
+  if (vec) rope_kernel<T, true, APPEND><<<grid, RA_WARPS * 32, 0, st>>>(prm);
+  else rope_kernel<T, false, APPEND><<<grid, RA_WARPS * 32, 0, st>>>(prm);
 }
 
 static int rope_run(const fa_rope_args_t* a, int append, const char* what, cudaStream_t st) {
@@ -278,7 +287,6 @@ static int rope_run(const fa_rope_args_t* a, int append, const char* what, cudaS
   }
   RopeParams prm;
   prm.a = *a;
-  prm.append = append;
   prm.lph_log2 = 0;
   while ((16 << prm.lph_log2) < a->D) ++prm.lph_log2;
   bool vec = a->Hq == 0 || (al16(a->q, a->q_st, a->q_sh) && al16(a->q_out, a->qo_st, a->qo_sh));
@@ -290,8 +298,17 @@ static int rope_run(const fa_rope_args_t* a, int append, const char* what, cudaS
     else
       vec = vec && al16(a->k_out, a->ko_st, a->ko_sh);
   }
-  if (a->dtype == FA_DTYPE_F16) rope_launch_t<__half>(prm, vec, st);
-  else rope_launch_t<__nv_bfloat16>(prm, vec, st);
+  // Two CTAs of 8 warps fill an SM.  From 16 tokens per SM on a warp takes tokens of its own, one after another; fewer are
+  // divided among more warps, down to one pass over the heads each, so that the walk's latency is not the call's.
+  const int groups = ceil_div(a->Hq + a->Hkv * (append ? 2 : 1), 32 >> prm.lph_log2);
+  const int full = 2 * RA_WARPS * sm_count();
+  prm.chunks = 1;
+  while (prm.chunks < groups && (int64_t)a->tokens * (prm.chunks + 1) <= full) ++prm.chunks;
+  const int unit = RA_WARPS * prm.chunks;             // whole tokens, whole CTAs
+  prm.warps = (int)(prm.chunks > 1 ? ceil_div64((int64_t)a->tokens * prm.chunks, unit) * unit
+                                   : (int64_t)RA_WARPS * ceil_div64(a->tokens < full ? a->tokens : full, RA_WARPS));
+  if (a->dtype == FA_DTYPE_F16) append ? rope_launch<__half, true>(prm, vec, st) : rope_launch<__half, false>(prm, vec, st);
+  else append ? rope_launch<__nv_bfloat16, true>(prm, vec, st) : rope_launch<__nv_bfloat16, false>(prm, vec, st);
   FA_CHECK_LAUNCH(what);
   return FA_OK;
 }
