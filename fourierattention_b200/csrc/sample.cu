@@ -6,12 +6,16 @@
 // The token is the first index i (ascending) whose running sum of kept weights exceeds u * (their sum).
 //
 // Nothing is sorted as a whole.  A head of the order is {x > t} plus the ties at t up to an index, so each of top-k and
-// top-p is a search for one element: a histogram of M - x over 1024 equal bins finds the bin it is in, the bin's
-// elements (up to LIST of them) are ranked against one another, and a fuller bin is split again, down to bins of one
-// value whose ties are counted in the order of their indices.  Whether a token is in hangs on sums next to a border,
-// and one token too many or too few changes the draw, so every sum that decides is taken in float64 in a fixed order;
-// the histogram of top-p (integers: the same whatever the order of the atomics) only proposes a bin, which the
-// float64 sums then confirm or move.
+// top-p is a search for one element.
+//   Small top-k (up to LIST): the k-th largest of the threads' own maxima is no larger than the k-th largest logit, so
+//   a histogram of those (one atomic per thread) gives a border above which all k are; what is above it, a little more
+//   than k, is listed and ranked by one CTA, which then cuts the list by top-p and min-p and draws from it.
+//   Else: a histogram of (largest - x) over 1024 equal bins finds the bin the element is in, the bin's elements (up to
+//   LIST of them) are ranked against one another, and a fuller bin is split again, down to bins of one value whose ties
+//   are counted in the order of their indices.
+// Whether a token is in hangs on sums next to a border, and one token too many or too few changes the draw, so every
+// weight and sum that decides is taken in float64, in a fixed order; the histogram of top-p (integers: the same whatever
+// the order of the atomics) only proposes a bin, which the float64 sums then confirm or move.
 //
 // Layout: a cluster of 1 to 8 CTAs holds a row in shared memory (float32, read from HBM once; a thread owns up
 // to 32 neighbouring elements, one word of padding per 32 keeps its walk free of bank conflicts) and exchanges partial
@@ -73,6 +77,30 @@ struct SaShared {
 };
 
 __device__ __forceinline__ double shfl_up_d(double v, int o) { return __shfl_up_sync(0xffffffffu, v, o); }
+// e^z for z <= 0, to a few units of 2^-53: z = n ln 2 + r with |r| <= ln 2 / 2 and n rounded by adding 1.5 * 2^52, the Taylor
+// polynomial of degree 12 (remainder (ln 2 / 2)^13 / 13! = 1.7e-16), and n added to the exponent.  Below e^-700: 0.
+__device__ __forceinline__ double sa_exp(double z) {
+  const double t = fma(z, 1.4426950408889634, 6755399441055744.0);
+  const int n = __double2loint(t);
+  const double nf = t - 6755399441055744.0;
+  double r = fma(nf, -0.6931471805599453, z);         // ln 2 as a sum of two doubles
+  r = fma(nf, -2.3190468138462996e-17, r);
+  double p = 1.0 / 479001600.0;
+  p = fma(p, r, 1.0 / 39916800.0);
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  const double e = __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
+  return z < -700.0 ? 0.0 : e;
+}
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -104,18 +132,25 @@ struct Sampler {
   int ki;
 
   __device__ __forceinline__ float& at(int i) { return xs[i + (i >> 5)]; }
-  __device__ __forceinline__ double weight(float x) const { return exp((double)(x - M) * inv_t); }
+  __device__ __forceinline__ double weight(float x) const { return sa_exp(((double)x - (double)M) * inv_t); }
   __device__ __forceinline__ bool kept(float x, int i) const { return x > kx || (x == kx && i <= ki); }
 
   template <typename F>
   __device__ __forceinline__ void each(F f) {
     for (int r = 0; r < p.rounds; ++r) {
       const int i0 = r * SA_ROUND + tid * p.ept, i1 = min(n, i0 + p.ept);
-      for (int i = i0; i < i1; ++i) f(at(i), base + i);
+      // four values are read before the first is used
+      for (int i = i0; i < i1; i += 4) {
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = i + k < i1 ? at(i + k) : -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f(v[k], base + i + k);
+      }
     }
   }
 
-  // sums over the cluster, in a fixed order: lanes, warps, CTAs.  Every CTA returns the same.
+  // Sums over the cluster, in a fixed order: lanes, warps, CTAs.  Every CTA returns the same.
   __device__ __forceinline__ void exchange(double s0, double s1, float mn, float mx, int n0, int n1, SaXchg& out) {
     s0 = warp_sum_d(s0), s1 = warp_sum_d(s1);
     mn = -warp_max(-mn), mx = warp_max(mx);
@@ -127,14 +162,13 @@ struct Sampler {
       sh.red_n[0][warp] = n0, sh.red_n[1][warp] = n1;
     }
     __syncthreads();
-    if (tid == 0) {
-      SaXchg o = {{0.0, 0.0}, {INFINITY, -INFINITY}, {0, 0}};
-      for (int w = 0; w < SA_WARPS; ++w) {
-        o.s[0] += sh.red_d[0][w], o.s[1] += sh.red_d[1][w];
-        o.f[0] = fminf(o.f[0], sh.red_f[0][w]), o.f[1] = fmaxf(o.f[1], sh.red_f[1][w]);
-        o.n[0] += sh.red_n[0][w], o.n[1] += sh.red_n[1][w];
-      }
-      sh.x[xb] = o;
+    if (warp == 0) {
+      const bool on = lane < SA_WARPS;
+      s0 = warp_sum_d(on ? sh.red_d[0][lane] : 0.0), s1 = warp_sum_d(on ? sh.red_d[1][lane] : 0.0);
+      mn = -warp_max(on ? -sh.red_f[0][lane] : -INFINITY), mx = warp_max(on ? sh.red_f[1][lane] : -INFINITY);
+      n0 = __reduce_add_sync(0xffffffffu, on ? sh.red_n[0][lane] : 0);
+      n1 = __reduce_add_sync(0xffffffffu, on ? sh.red_n[1][lane] : 0);
+      if (lane == 0) sh.x[xb] = SaXchg{{s0, s1}, {mn, mx}, {n0, n1}};
     }
     cl.sync();
     out = {{0.0, 0.0}, {INFINITY, -INFINITY}, {0, 0}};
@@ -272,8 +306,8 @@ struct Sampler {
       }
       if (by_weight) {
         // relative to the weight at hi
-        v0 *= exp((double)(2 * tid * width) * -inv_t);
-        v1 *= exp((double)((2 * tid + 1) * width) * -inv_t);
+        v0 *= sa_exp((double)(2 * tid * width) * -inv_t);
+        v1 *= sa_exp((double)((2 * tid + 1) * width) * -inv_t);
       }
       double pre = v0 + v1;              // running sum up to and with this thread's bins
 #pragma unroll
@@ -345,7 +379,7 @@ struct Sampler {
           return;
         }
         if (o.n[1] <= SA_LIST) {
-          rank_list(o.n[1], by_weight, k - o.n[0], o.s[0], goal);
+          cut_list(o.n[1], by_weight, k - o.n[0], o.s[0], goal);
           return;
         }
         lo = o.f[0], hi = o.f[1];
@@ -374,8 +408,8 @@ struct Sampler {
     kx = x;
   }
 
-  // orders the n listed elements of the cluster and cuts the kept head at one of them
-  __device__ void rank_list(int n_all, bool by_weight, int k, double before, double goal) {
+  // the listed elements of the cluster, in order: ox, oi, and their weights in gw
+  __device__ void rank_list(int n_all, bool weights) {
     int off = 0;
     for (int r = 0; r < size; ++r) {
       const int c = (int)*cl.map_shared_rank(&sh.ln, r);
@@ -386,37 +420,127 @@ struct Sampler {
       off += c;
     }
     __syncthreads();
-    for (int e = tid; e < n_all; e += SA_THREADS) {
-      const float x = sh.gx[e];
-      const int i = sh.gi[e];
+    if (tid < n_all) {
+      const float x = sh.gx[tid];
+      const int i = sh.gi[tid];
       int rk = 0;
+#pragma unroll 4
       for (int j = 0; j < n_all; ++j) rk += sh.gx[j] > x || (sh.gx[j] == x && sh.gi[j] < i);
       sh.ox[rk] = x, sh.oi[rk] = i;
-      sh.gw[rk] = by_weight ? weight(x) : 0.0;
+      sh.gw[rk] = weights ? weight(x) : 0.0;
     }
-    if (tid == 0) sh.pick = n_all - 1;
     __syncthreads();
-    if (by_weight) {
-      // running sum over at most SA_THREADS elements, one per thread
-      double inc = tid < n_all ? sh.gw[tid] : 0.0;
+  }
+  // running sum of one value per thread, and the sum of all
+  __device__ double block_scan(double v, double& total) {
+    double inc = v;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double v = shfl_up_d(inc, o);
-        if (lane >= o) inc += v;
-      }
-      if (lane == 31) sh.red_d[0][warp] = inc;
-      __syncthreads();
-      double pre = before;
-      for (int w = 0; w < warp; ++w) pre += sh.red_d[0][w];
-      if (tid < n_all && pre + inc >= goal) atomicMin(&sh.pick, tid);
-      __syncthreads();
-    } else if (tid == 0) {
-      sh.pick = max(0, min(k - 1, n_all - 1));
+    for (int o = 1; o < 32; o <<= 1) {
+      const double x = shfl_up_d(inc, o);
+      if (lane >= o) inc += x;
     }
     __syncthreads();
-    kx = sh.ox[sh.pick];
-    ki = sh.oi[sh.pick];
+    if (lane == 31) sh.red_d[0][warp] = inc;
     __syncthreads();
+    double pre = 0.0;
+    total = 0.0;
+#pragma unroll
+    for (int w = 0; w < SA_WARPS; ++w) {
+      const double x = sh.red_d[0][w];
+      if (w < warp) pre += x;
+      total += x;
+    }
+    return pre + inc;
+  }
+  // cuts the kept head at the k-th of the n listed elements, or at the first where the running sum reaches the goal
+  __device__ void cut_list(int n_all, bool by_weight, int k, double before, double goal) {
+    rank_list(n_all, by_weight);
+    int last = max(0, min(k - 1, n_all - 1));
+    if (by_weight) {
+      if (tid == 0) sh.pick = n_all - 1;
+      double total;
+      const double inc = block_scan(tid < n_all ? sh.gw[tid] : 0.0, total);
+      if (tid < n_all && before + inc >= goal) atomicMin(&sh.pick, tid);
+      __syncthreads();
+      last = sh.pick;
+    }
+    kx = sh.ox[last];
+    ki = sh.oi[last];
+    __syncthreads();
+  }
+
+  // Small top-k: true if the token has been drawn.  `mine` is the largest of the logits this thread has read.
+  __device__ bool draw_short(int row, int k, float mine, float low, float top_p, double min_p, double u) {
+    const float half = M - low < INFINITY ? 1.f : 0.5f;
+    const float top = half * M, range = top - half * low, scale = (float)SA_BINS / range;
+    auto bin_of = [&](float x) { return min(SA_BINS - 1, (int)(fmaf(-half, x, top) * scale)); };
+    for (int i = tid; i < SA_BINS; i += SA_THREADS) sh.hist[i] = 0;
+    if (tid == 0) sh.pick = SA_BINS, sh.ln = 0;
+    __syncthreads();
+    if (mine > -INFINITY) atomicAdd(&sh.hist[bin_of(mine)], 1u);
+    cl.sync();
+    int v0 = 0, v1 = 0;                  // two neighbouring bins per thread, over the cluster
+    for (int r = 0; r < size; ++r) {
+      const uint2 h = *reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh.hist[2 * tid], r));
+      v0 += (int)h.x, v1 += (int)h.y;
+    }
+    int pre = v0 + v1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, pre, o);
+      if (lane >= o) pre += v;
+    }
+    if (lane == 31) sh.red_n[0][warp] = pre;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < SA_WARPS; ++w)
+      if (w < warp) pre += sh.red_n[0][w];
+    pre -= v0 + v1;
+    if (v0 > 0 && pre + v0 >= k) atomicMin(&sh.pick, 2 * tid);
+    else if (v1 > 0 && pre + v0 + v1 >= k) atomicMin(&sh.pick, 2 * tid + 1);
+    __syncthreads();
+    const int b = sh.pick;
+    if (b >= SA_BINS) return false;      // fewer threads with logits than k
+    each([&](float x, int i) {
+      if (x > -INFINITY && bin_of(x) <= b) {
+        const unsigned slot = atomicAdd(&sh.ln, 1u);
+        if (slot < SA_LIST) sh.lx[slot] = x, sh.li[slot] = i;
+      }
+    });
+    cl.sync();
+    int n_all = 0;
+    for (int r = 0; r < size; ++r) n_all += (int)*cl.map_shared_rank(&sh.ln, r);
+    if (n_all > SA_LIST) {
+      cl.sync();                         // the lists are written anew
+      return false;
+    }
+    if (rank != 0) return true;
+    // ---- the k largest, in order, one per thread -----------------------------------------------------------------------
+    rank_list(n_all, true);
+    const double w = tid < k ? sh.gw[tid] : 0.0;
+    double total;
+    const double inc = block_scan(w, total);
+    const bool keep = tid == 0 || (tid < k && w >= min_p && (top_p >= 1.f || inc - w < (double)fmaxf(top_p, 0.f) * total));
+    const int n_keep = __syncthreads_count(keep);      // a head of the order, as each of the three is
+    double kept_sum;
+    block_scan(tid < n_keep ? w : 0.0, kept_sum);
+    if (tid == 0) sh.pick = 0x7fffffff, sh.pick_i = -1;
+    __syncthreads();
+    if (tid < n_keep && w > 0.0) {
+      const int i = sh.oi[tid];
+      double run_sum = 0.0;              // of the kept weights up to this index
+#pragma unroll 4
+      for (int j = 0; j < n_keep; ++j) run_sum += sh.oi[j] <= i ? sh.gw[j] : 0.0;
+      if (run_sum > u * kept_sum) atomicMin(&sh.pick, i);
+      atomicMax(&sh.pick_i, i);          // the last one, for u -> 1
+    }
+    __syncthreads();
+    const int token = sh.pick == 0x7fffffff ? sh.pick_i : sh.pick;
+    if (tid < n_keep && sh.oi[tid] == token) {
+      p.token[row] = token;
+      if (p.logprob) p.logprob[row] = (float)log(w / kept_sum);
+    }
+    return true;
   }
 
   __device__ void run(int row) {
@@ -479,33 +603,46 @@ struct Sampler {
       // the limit of ever larger logits: those at +infinity share the probability
       int c = 0;
       for (int i = tid; i < n; i += SA_THREADS) {
-        at(i) = at(i) == INFINITY ? 0.f : -INFINITY;
-        c += at(i) == 0.f;
+        const float v = at(i) == INFINITY ? 0.f : -INFINITY;
+        at(i) = v;
+        c += v == 0.f;
       }
       exchange(0.0, 0.0, 0.f, 0.f, c, 0, o);
       M = 0.f, low = 0.f, n_fin = o.n[0];
     }
     inv_t = temperature > 0.f ? 1.0 / (double)temperature : 0.0;
-    if (!(temperature > 0.f)) top_k = 1;   // the largest logit, lowest index
+    if (!(temperature > 0.f)) top_k = 1;
+    const double u = (double)p.u[row];
+    if (top_k == 1) {
+      // the largest logit, lowest index
+      const int first = nth_tie(M, 0);
+      if (rank == 0 && tid == 0) {
+        p.token[row] = first;
+        if (p.logprob) p.logprob[row] = 0.f;
+      }
+      return;
+    }
+    if (top_k > 0 && top_k <= SA_LIST && top_k < n_fin && M > low && draw_short(row, top_k, mx, low, top_p, (double)min_p, u))
+      return;
     if (top_k > 0 && top_k < n_fin) shorten(false, top_k, 0.0, 0.0, low, M);
-    if (top_p < 1.f && top_k != 1) {
+    if (top_p < 1.f) {
       double s = 0.0;
       each([&](float v, int i) {
-        if (kept(v, i)) s += weight(v);
+        const double w = weight(v);
+        s += kept(v, i) ? w : 0.0;
       });
       exchange(s, 0.0, 0.f, 0.f, 0, 0, o);
       shorten(true, 0, (double)fmaxf(top_p, 0.f) * o.s[0], o.s[0], kx > -INFINITY ? kx : low, M);
     }
-    draw(row, (double)p.u[row], (double)min_p);
+    draw(row, u, (double)min_p);
   }
 
   __device__ void draw(int row, double u, double min_p) {
     double W = 0.0;
     auto mass = [&](int i) -> double {
       const float v = at(i);
-      if (!kept(v, base + i)) return 0.0;
       const double w = weight(v);
-      return w >= min_p || v == M ? w : 0.0;
+      return kept(v, base + i) && (w >= min_p || v == M) ? w : 0.0;
     };
     double mine[SA_MAX_ROUNDS], s = 0.0;
 #pragma unroll
@@ -513,7 +650,13 @@ struct Sampler {
       mine[r] = 0.0;
       if (r >= p.rounds) continue;
       const int i0 = r * SA_ROUND + tid * p.ept, i1 = min(n, i0 + p.ept);
-      for (int i = i0; i < i1; ++i) mine[r] += mass(i);
+      for (int i = i0; i < i1; i += 4) {
+        double w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = i + k < i1 ? mass(i + k) : 0.0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mine[r] += w[k];
+      }
       s += mine[r];
     }
     // the CTA's sum, and those of the CTAs before it
@@ -616,7 +759,7 @@ struct Sampler {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(SA_THREADS) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleParams p) {
   extern __shared__ float sa_xs[];
   __shared__ SaShared sh;
   cg::cluster_group cl = cg::this_cluster();
