@@ -63,11 +63,8 @@ struct SaShared {
   float lx[SA_LIST];          // this CTA's part of a bin
   int li[SA_LIST];
   unsigned ln;
-  float gx[SA_LIST];          // the bin of the whole cluster
-  int gi[SA_LIST];
-  double gw[SA_LIST];         // its weights, in order
-  float ox[SA_LIST];
-  int oi[SA_LIST];
+  unsigned long long key[SA_LIST];   // the bin of the whole cluster
+  double gw[SA_LIST];
   double red_d[2][SA_WARPS];
   float red_f[2][SA_WARPS];
   int red_n[2][SA_WARPS];
@@ -110,11 +107,11 @@ __device__ __forceinline__ double warp_sum_d(double v) {
 template <typename T>
 __device__ __forceinline__ float sa_value(T v) {
   const float f = to_f32(v);
-  return f != f ? -INFINITY : f;       // NaN: never drawn
+  return f != f ? -INFINITY : f + 0.f;       // NaN: never drawn; the two zeros are equal
 }
 template <>
 __device__ __forceinline__ float sa_value<float>(float f) {
-  return f != f ? -INFINITY : f;
+  return f != f ? -INFINITY : f + 0.f;
 }
 
 template <typename T>
@@ -150,6 +147,33 @@ struct Sampler {
     }
   }
 
+  // f(logit, index, weight) for the elements that `want` takes: first which they are, then their weights, two at a time,
+  // so that a warp computes as many as its busiest lane has, not one for every element that some lane has
+  template <typename P, typename F>
+  __device__ __forceinline__ void each_weight(P want, F f) {
+    for (int r = 0; r < p.rounds; ++r) {
+      const int i0 = r * SA_ROUND + tid * p.ept, c = min(n - i0, p.ept);
+      unsigned mask = 0;
+      for (int i = 0; i < c; i += 4) {
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = i + k < c ? at(i0 + i + k) : -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mask |= (unsigned)want(v[k], base + i0 + i + k) << (i + k);
+      }
+      while (mask) {
+        const int a = __ffs(mask) - 1;
+        mask &= mask - 1;
+        const int b = mask ? __ffs(mask) - 1 : -1;
+        mask &= mask - 1;
+        const float xa = at(i0 + a), xb = b >= 0 ? at(i0 + b) : xa;
+        const double wa = weight(xa), wb = weight(xb);
+        f(xa, base + i0 + a, wa);
+        if (b >= 0) f(xb, base + i0 + b, wb);
+      }
+    }
+  }
+
   // Sums over the cluster, in a fixed order: lanes, warps, CTAs.  Every CTA returns the same.
   __device__ __forceinline__ void exchange(double s0, double s1, float mn, float mx, int n0, int n1, SaXchg& out) {
     s0 = warp_sum_d(s0), s1 = warp_sum_d(s1);
@@ -171,14 +195,32 @@ struct Sampler {
       if (lane == 0) sh.x[xb] = SaXchg{{s0, s1}, {mn, mx}, {n0, n1}};
     }
     cl.sync();
-    out = {{0.0, 0.0}, {INFINITY, -INFINITY}, {0, 0}};
-    for (int r = 0; r < size; ++r) {
-      const SaXchg o = *cl.map_shared_rank(&sh.x[xb], r);
-      out.s[0] += o.s[0], out.s[1] += o.s[1];
-      out.f[0] = fminf(out.f[0], o.f[0]), out.f[1] = fmaxf(out.f[1], o.f[1]);
-      out.n[0] += o.n[0], out.n[1] += o.n[1];
+    // a lane per CTA
+    out = SaXchg{{0.0, 0.0}, {INFINITY, -INFINITY}, {0, 0}};
+    if (lane < size) out = *cl.map_shared_rank(&sh.x[xb], lane);
+#pragma unroll
+    for (int o = SA_MAX_CLUSTER / 2; o > 0; o >>= 1) {
+      out.s[0] += __shfl_xor_sync(0xffffffffu, out.s[0], o), out.s[1] += __shfl_xor_sync(0xffffffffu, out.s[1], o);
+      out.f[0] = fminf(out.f[0], __shfl_xor_sync(0xffffffffu, out.f[0], o));
+      out.f[1] = fmaxf(out.f[1], __shfl_xor_sync(0xffffffffu, out.f[1], o));
+      out.n[0] += __shfl_xor_sync(0xffffffffu, out.n[0], o), out.n[1] += __shfl_xor_sync(0xffffffffu, out.n[1], o);
     }
+    out.s[0] = __shfl_sync(0xffffffffu, out.s[0], 0), out.s[1] = __shfl_sync(0xffffffffu, out.s[1], 0);
+    out.f[0] = __shfl_sync(0xffffffffu, out.f[0], 0), out.f[1] = __shfl_sync(0xffffffffu, out.f[1], 0);
+    out.n[0] = __shfl_sync(0xffffffffu, out.n[0], 0), out.n[1] = __shfl_sync(0xffffffffu, out.n[1], 0);
     xb ^= 1;
+  }
+  // this thread's two bins of the histogram, over the cluster
+  __device__ __forceinline__ void read_bins(unsigned& a, unsigned& b) {
+    uint2 h[SA_MAX_CLUSTER];
+#pragma unroll
+    for (int r = 0; r < SA_MAX_CLUSTER; ++r) {
+      h[r] = make_uint2(0, 0);
+      if (r < size) h[r] = *reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh.hist[2 * tid], r));
+    }
+    a = b = 0;
+#pragma unroll
+    for (int r = 0; r < SA_MAX_CLUSTER; ++r) a += h[r].x, b += h[r].y;
   }
 
   // index of the m-th (from 0) element equal to x in the order of the indices
@@ -277,8 +319,8 @@ struct Sampler {
   }
 
   // Shortens the kept head: to its first `k` elements (by_weight false), or to the shortest one whose weight reaches
-  // `goal` (by_weight true; `part` is the weight of the whole kept head).  Its logits are in [lo, hi].
-  __device__ void shorten(bool by_weight, int k, double goal, double part, float lo, float hi) {
+  // `goal` (by_weight true).  The element it ends with is in [lo, hi].
+  __device__ void shorten(bool by_weight, int k, double goal, float lo, float hi) {
     double near = 0.0;                 // what lies above hi: a number of elements or a weight
     for (int level = 0; level < 256; ++level) {
       // a bin number that never falls with hi - x, whatever the rounding; 0 for hi and the last one for lo, so that
@@ -293,39 +335,23 @@ struct Sampler {
       each([&](float x, int i) {
         if (!kept(x, i) || x > hi || x < lo) return;
         const int b = bin_of(x);
-        // weights relative to the bin's near edge, in steps of 2^-14: a CTA's part of a bin stays below 2^30
+        // weights relative to the bin's near edge, in steps of 2^-14; a bin may hold 2^18 of the largest
         const float rel = fminf(0.f, (x - hi + (float)b * width) * c_w);
         atomicAdd(&sh.hist[b], by_weight ? max(1u, __float2uint_rn(16384.f * __expf(rel))) : 1u);
       });
       cl.sync();
       // two neighbouring bins per thread, over the cluster
-      double v0 = 0.0, v1 = 0.0;
-      for (int r = 0; r < size; ++r) {
-        const uint2 h = *reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh.hist[2 * tid], r));
-        v0 += (double)h.x, v1 += (double)h.y;
-      }
+      unsigned h0, h1;
+      read_bins(h0, h1);
+      double v0 = (double)h0, v1 = (double)h1;
       if (by_weight) {
         // relative to the weight at hi
         v0 *= sa_exp((double)(2 * tid * width) * -inv_t);
         v1 *= sa_exp((double)((2 * tid + 1) * width) * -inv_t);
       }
-      double pre = v0 + v1;              // running sum up to and with this thread's bins
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double v = shfl_up_d(pre, o);
-        if (lane >= o) pre += v;
-      }
-      __syncthreads();
-      if (lane == 31) sh.red_d[0][warp] = pre;
-      __syncthreads();
-      double total = 0.0;
-      for (int w = 0; w < SA_WARPS; ++w) {
-        if (w < warp) pre += sh.red_d[0][w];
-        total += sh.red_d[0][w];
-      }
-      pre -= v0 + v1;
-      // the histogram's weights are in units of their own, `unit` of them make one of the exact sums
-      const double unit = by_weight ? total / part : 1.0;
+      double total, pre = block_scan(v0 + v1, total) - (v0 + v1);   // what lies before this thread's bins
+      // the histogram counts weights in units of 2^-14 of the weight at hi
+      const double unit = by_weight ? 16384.0 / weight(hi) : 1.0;
       double target = by_weight ? fmin((goal - near) * unit, total) : (double)k - near;
 
       // ---- the bin's elements, and what lies before it --------------------------------------------------------
@@ -343,12 +369,8 @@ struct Sampler {
         double s_before = 0.0, s_in = 0.0;
         float mn = INFINITY, mx = -INFINITY;
         int n_in = 0, n_before = 0;
-        each([&](float x, int i) {
-          if (!kept(x, i) || x < lo) return;
-          const int bb = x > hi ? -1 : bin_of(x);
-          if (bb > b) return;
-          const double w = by_weight ? weight(x) : 0.0;
-          if (bb < b) {
+        auto take = [&](float x, int i, double w) {
+          if (x > hi || bin_of(x) < b) {
             s_before += w;
             ++n_before;
           } else {
@@ -358,6 +380,11 @@ struct Sampler {
             const unsigned slot = atomicAdd(&sh.ln, 1u);
             if (slot < SA_LIST) sh.lx[slot] = x, sh.li[slot] = i;
           }
+        };
+        auto want = [&](float x, int i) { return kept(x, i) && x >= lo && (x > hi || bin_of(x) <= b); };
+        if (by_weight) each_weight(want, take);
+        else each([&](float x, int i) {
+          if (want(x, i)) take(x, i, 0.0);
         });
         SaXchg o;
         exchange(s_before, s_in, mn, mx, n_before, n_in, o);
@@ -384,7 +411,6 @@ struct Sampler {
         }
         lo = o.f[0], hi = o.f[1];
         near = by_weight ? o.s[0] : (double)o.n[0];
-        part = o.s[1];
         split = true;
         break;
       }
@@ -408,28 +434,49 @@ struct Sampler {
     kx = x;
   }
 
-  // the listed elements of the cluster, in order: ox, oi, and their weights in gw
-  __device__ void rank_list(int n_all, bool weights) {
-    int off = 0;
-    for (int r = 0; r < size; ++r) {
-      const int c = (int)*cl.map_shared_rank(&sh.ln, r);
-      for (int i = tid; i < c; i += SA_THREADS) {
-        sh.gx[off + i] = *cl.map_shared_rank(&sh.lx[i], r);
-        sh.gi[off + i] = *cl.map_shared_rank(&sh.li[i], r);
+  // larger logits first, lower indices first among equals: ascending
+  static __device__ __forceinline__ unsigned long long key_of(float x, int i) {
+    const unsigned u = __float_as_uint(x);
+    return ((unsigned long long)((u >> 31) ? u : ~(u | 0x80000000u)) << 32) | (unsigned)i;
+  }
+  static __device__ __forceinline__ float key_value(unsigned long long k) {
+    const unsigned u = (unsigned)(k >> 32);
+    return __uint_as_float((u >> 31) ? u : ~(u | 0x80000000u));
+  }
+  // ascending order of one key per thread, the first n of which count (a bitonic network: within warps by shuffles)
+  __device__ unsigned long long sort_keys(unsigned long long k, int n_all) {
+    int n2 = 32;
+    while (n2 < n_all) n2 *= 2;
+    for (int len = 2; len <= n2; len *= 2)
+      for (int o = len / 2; o > 0; o /= 2) {
+        unsigned long long other;
+        if (o >= 32) {
+          __syncthreads();
+          sh.key[tid] = k;
+          __syncthreads();
+          other = sh.key[tid ^ o];
+        } else {
+          other = __shfl_xor_sync(0xffffffffu, k, o);
+        }
+        const bool low = (tid & o) == 0, up = (tid & len) == 0 || len == n2;
+        k = (low == up) == (other < k) ? other : k;
       }
+    return k;
+  }
+  // the listed elements of the cluster, in order, one per thread
+  __device__ unsigned long long sorted_list(int n_all) {
+    static_assert(SA_LIST == SA_THREADS, "an element per thread");
+    const int mine = lane < size ? (int)*cl.map_shared_rank(&sh.ln, lane) : 0;
+    unsigned long long k = ~0ull;
+    int off = 0;
+#pragma unroll
+    for (int r = 0; r < SA_MAX_CLUSTER; ++r) {
+      const int c = __shfl_sync(0xffffffffu, mine, r);
+      if (tid >= off && tid < off + c)
+        k = key_of(*cl.map_shared_rank(&sh.lx[tid - off], r), *cl.map_shared_rank(&sh.li[tid - off], r));
       off += c;
     }
-    __syncthreads();
-    if (tid < n_all) {
-      const float x = sh.gx[tid];
-      const int i = sh.gi[tid];
-      int rk = 0;
-#pragma unroll 4
-      for (int j = 0; j < n_all; ++j) rk += sh.gx[j] > x || (sh.gx[j] == x && sh.gi[j] < i);
-      sh.ox[rk] = x, sh.oi[rk] = i;
-      sh.gw[rk] = weights ? weight(x) : 0.0;
-    }
-    __syncthreads();
+    return sort_keys(k, n_all);
   }
   // running sum of one value per thread, and the sum of all
   __device__ double block_scan(double v, double& total) {
@@ -454,18 +501,22 @@ struct Sampler {
   }
   // cuts the kept head at the k-th of the n listed elements, or at the first where the running sum reaches the goal
   __device__ void cut_list(int n_all, bool by_weight, int k, double before, double goal) {
-    rank_list(n_all, by_weight);
-    int last = max(0, min(k - 1, n_all - 1));
+    const unsigned long long key = sorted_list(n_all);
+    __syncthreads();
+    if (tid == 0) sh.pick = n_all - 1;
+    __syncthreads();
     if (by_weight) {
-      if (tid == 0) sh.pick = n_all - 1;
       double total;
-      const double inc = block_scan(tid < n_all ? sh.gw[tid] : 0.0, total);
+      const double inc = block_scan(tid < n_all ? weight(key_value(key)) : 0.0, total);
       if (tid < n_all && before + inc >= goal) atomicMin(&sh.pick, tid);
-      __syncthreads();
-      last = sh.pick;
+    } else if (tid == 0) {
+      sh.pick = max(0, min(k - 1, n_all - 1));
     }
-    kx = sh.ox[last];
-    ki = sh.oi[last];
+    __syncthreads();
+    if (tid == sh.pick) sh.key[0] = key;
+    __syncthreads();
+    kx = key_value(sh.key[0]);
+    ki = (int)(unsigned)sh.key[0];
     __syncthreads();
   }
 
@@ -479,11 +530,9 @@ struct Sampler {
     __syncthreads();
     if (mine > -INFINITY) atomicAdd(&sh.hist[bin_of(mine)], 1u);
     cl.sync();
-    int v0 = 0, v1 = 0;                  // two neighbouring bins per thread, over the cluster
-    for (int r = 0; r < size; ++r) {
-      const uint2 h = *reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh.hist[2 * tid], r));
-      v0 += (int)h.x, v1 += (int)h.y;
-    }
+    unsigned h0, h1;
+    read_bins(h0, h1);
+    const int v0 = (int)h0, v1 = (int)h1;
     int pre = v0 + v1;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -508,37 +557,36 @@ struct Sampler {
       }
     });
     cl.sync();
-    int n_all = 0;
-    for (int r = 0; r < size; ++r) n_all += (int)*cl.map_shared_rank(&sh.ln, r);
+    const int n_all = __reduce_add_sync(0xffffffffu, lane < size ? (int)*cl.map_shared_rank(&sh.ln, lane) : 0);
     if (n_all > SA_LIST) {
       cl.sync();                         // the lists are written anew
       return false;
     }
     if (rank != 0) return true;
     // ---- the k largest, in order, one per thread -----------------------------------------------------------------------
-    rank_list(n_all, true);
-    const double w = tid < k ? sh.gw[tid] : 0.0;
-    double total;
+    const unsigned long long key = sorted_list(n_all);
+    const int index = (int)(unsigned)key;
+    const double w = tid < k ? weight(key_value(key)) : 0.0;
+    double total, kept_sum;
     const double inc = block_scan(w, total);
     const bool keep = tid == 0 || (tid < k && w >= min_p && (top_p >= 1.f || inc - w < (double)fmaxf(top_p, 0.f) * total));
     const int n_keep = __syncthreads_count(keep);      // a head of the order, as each of the three is
-    double kept_sum;
-    block_scan(tid < n_keep ? w : 0.0, kept_sum);
-    if (tid == 0) sh.pick = 0x7fffffff, sh.pick_i = -1;
+    // the kept ones in the order of their indices
+    sh.gw[tid] = tid < n_keep ? w : 0.0;
+    const unsigned long long by_index = sort_keys(tid < n_keep ? ((unsigned long long)index << 32) | (unsigned)tid : ~0ull, n_keep);
     __syncthreads();
-    if (tid < n_keep && w > 0.0) {
-      const int i = sh.oi[tid];
-      double run_sum = 0.0;              // of the kept weights up to this index
-#pragma unroll 4
-      for (int j = 0; j < n_keep; ++j) run_sum += sh.oi[j] <= i ? sh.gw[j] : 0.0;
-      if (run_sum > u * kept_sum) atomicMin(&sh.pick, i);
-      atomicMax(&sh.pick_i, i);          // the last one, for u -> 1
+    const double wi = tid < n_keep ? sh.gw[(unsigned)by_index & (SA_LIST - 1)] : 0.0;
+    const double run_sum = block_scan(wi, kept_sum);
+    if (tid == 0) sh.pick = SA_LIST, sh.pick_i = -1;
+    __syncthreads();
+    if (wi > 0.0) {
+      if (run_sum > u * kept_sum) atomicMin(&sh.pick, tid);
+      atomicMax(&sh.pick_i, tid);        // the last one, for u -> 1
     }
     __syncthreads();
-    const int token = sh.pick == 0x7fffffff ? sh.pick_i : sh.pick;
-    if (tid < n_keep && sh.oi[tid] == token) {
-      p.token[row] = token;
-      if (p.logprob) p.logprob[row] = (float)log(w / kept_sum);
+    if (tid == (sh.pick < SA_LIST ? sh.pick : sh.pick_i)) {
+      p.token[row] = (int64_t)(by_index >> 32);
+      if (p.logprob) p.logprob[row] = (float)log(wi / kept_sum);
     }
     return true;
   }
@@ -624,15 +672,15 @@ struct Sampler {
     }
     if (top_k > 0 && top_k <= SA_LIST && top_k < n_fin && M > low && draw_short(row, top_k, mx, low, top_p, (double)min_p, u))
       return;
-    if (top_k > 0 && top_k < n_fin) shorten(false, top_k, 0.0, 0.0, low, M);
+    if (top_k > 0 && top_k < n_fin) shorten(false, top_k, 0.0, low, M);
     if (top_p < 1.f) {
       double s = 0.0;
-      each([&](float v, int i) {
-        const double w = weight(v);
-        s += kept(v, i) ? w : 0.0;
-      });
+      each_weight([&](float v, int i) { return kept(v, i); }, [&](float, int, double w) { s += w; });
       exchange(s, 0.0, 0.f, 0.f, 0, 0, o);
-      shorten(true, 0, (double)fmaxf(top_p, 0.f) * o.s[0], o.s[0], kx > -INFINITY ? kx : low, M);
+      // logits so low that all of them together weigh less than half of what top-p drops are not where it ends
+      const double p0 = (double)fmaxf(top_p, 0.f);
+      const float from = (float)((double)M + log(0.5 * (1.0 - p0) * o.s[0] / (double)n_fin) / inv_t);
+      shorten(true, 0, p0 * o.s[0], fmaxf(kx > -INFINITY ? kx : low, fminf(from, M)), M);
     }
     draw(row, u, (double)min_p);
   }
@@ -641,24 +689,21 @@ struct Sampler {
     double W = 0.0;
     auto mass = [&](int i) -> double {
       const float v = at(i);
+      if (!kept(v, base + i)) return 0.0;
       const double w = weight(v);
-      return kept(v, base + i) && (w >= min_p || v == M) ? w : 0.0;
+      return w >= min_p || v == M ? w : 0.0;
     };
-    double mine[SA_MAX_ROUNDS], s = 0.0;
+    double mine[SA_MAX_ROUNDS] = {0.0, 0.0, 0.0}, s = 0.0;
+    each_weight([&](float v, int i) { return kept(v, i); },
+                [&](float v, int i, double w) {
+                  const int r = (i - base) / SA_ROUND;
+                  if (w >= min_p || v == M) {
 #pragma unroll
-    for (int r = 0; r < SA_MAX_ROUNDS; ++r) {
-      mine[r] = 0.0;
-      if (r >= p.rounds) continue;
-      const int i0 = r * SA_ROUND + tid * p.ept, i1 = min(n, i0 + p.ept);
-      for (int i = i0; i < i1; i += 4) {
-        double w[4];
+                    for (int x = 0; x < SA_MAX_ROUNDS; ++x) mine[x] += x == r ? w : 0.0;
+                  }
+                });
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = i + k < i1 ? mass(i + k) : 0.0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mine[r] += w[k];
-      }
-      s += mine[r];
-    }
+    for (int r = 0; r < SA_MAX_ROUNDS; ++r) s += mine[r];
     // the CTA's sum, and those of the CTAs before it
     s = warp_sum_d(s);
     __syncthreads();
@@ -671,15 +716,18 @@ struct Sampler {
       sh.x[xb].s[0] = t;
     }
     cl.sync();
-    double pre = 0.0;
-    int owner = 0;
-    double own_pre = 0.0;
-    for (int r = 0; r < size; ++r) W += cl.map_shared_rank(&sh.x[xb], r)->s[0];
+    const double share = lane < size ? cl.map_shared_rank(&sh.x[xb], lane)->s[0] : 0.0;
+#pragma unroll
+    for (int r = 0; r < SA_MAX_CLUSTER; ++r) W += __shfl_sync(0xffffffffu, share, r);
     const double goal = u * W;
-    for (int r = 0; r < size; ++r) {
-      const double c = cl.map_shared_rank(&sh.x[xb], r)->s[0];
-      if (c > 0.0) owner = r, own_pre = pre;         // the last CTA with weight, unless one before it passes the goal
-      if (pre + c > goal) break;
+    double pre = 0.0, own_pre = 0.0;
+    int owner = 0;
+    bool found = false;
+#pragma unroll
+    for (int r = 0; r < SA_MAX_CLUSTER; ++r) {
+      const double c = __shfl_sync(0xffffffffu, share, r);
+      if (c > 0.0 && !found) owner = r, own_pre = pre;   // the last CTA with weight, unless one before it passes the goal
+      if (pre + c > goal) found = true;
       pre += c;
     }
     xb ^= 1;
