@@ -18,7 +18,8 @@
 // the order of the atomics) only proposes a bin, which the float64 sums then confirm or move.
 //
 // Layout: a cluster of 1 to 8 CTAs holds a row in shared memory (float32, read from HBM once; a thread owns up
-// to 32 neighbouring elements, one word of padding per 32 keeps its walk free of bank conflicts) and exchanges partial
+// to 32 neighbouring elements, read four at a time, its groups of four turned by its number so that a walk meets no bank
+// twice) and exchanges partial
 // results through distributed shared memory: every CTA reads all of them and decides alike, one cluster barrier per
 // step.  Bound: latency of those steps for few rows, issue of the float64 exponentials for many.
 #include <cooperative_groups.h>
@@ -42,7 +43,7 @@ constexpr int SA_MAX_VOCAB = SA_MAX_CLUSTER * SA_MAX_ROUNDS * SA_ROUND;
 struct SampleParams {
   const void* logits;
   int64_t sb;
-  int V, slice, ept, rounds;      // elements of a CTA, of a thread per round; rounds of SA_ROUND elements
+  int V, slice, ept_log2, rounds; // elements of a CTA, of a thread per round; rounds of 512 threads
   const float *u, *temperature, *top_p, *min_p;    // per row, or null: the value below
   const int32_t* top_k;
   float temperature0, top_p0, min_p0;
@@ -58,6 +59,7 @@ struct SaXchg {
 };
 
 struct SaShared {
+  double exp2[64];            // 2^(i / 64)
   uint32_t hist[SA_BINS];
   SaXchg x[2];
   float lx[SA_LIST];          // this CTA's part of a bin
@@ -74,28 +76,22 @@ struct SaShared {
 };
 
 __device__ __forceinline__ double shfl_up_d(double v, int o) { return __shfl_up_sync(0xffffffffu, v, o); }
-// e^z for z <= 0, to a few units of 2^-53: z = n ln 2 + r with |r| <= ln 2 / 2 and n rounded by adding 1.5 * 2^52, the Taylor
-// polynomial of degree 12 (remainder (ln 2 / 2)^13 / 13! = 1.7e-16), and n added to the exponent.  Below e^-700: 0.
-__device__ __forceinline__ double sa_exp(double z) {
-  const double t = fma(z, 1.4426950408889634, 6755399441055744.0);
+// e^z for z <= 0, to a few units of 2^-53: z = (n / 64) ln 2 + r with |r| <= ln 2 / 128 and n rounded by adding
+// 1.5 * 2^52; 2^((n mod 64) / 64) from a table, the Taylor polynomial of degree 5 (remainder r^6 / 720 = 4e-17), n / 64
+// added to the exponent.  Below e^-700: 0.
+__device__ __forceinline__ double sa_exp(double z, const double* table) {
+  const double t = fma(z, 64.0 * 1.4426950408889634, 6755399441055744.0);
   const int n = __double2loint(t);
   const double nf = t - 6755399441055744.0;
-  double r = fma(nf, -0.6931471805599453, z);         // ln 2 as a sum of two doubles
-  r = fma(nf, -2.3190468138462996e-17, r);
-  double p = 1.0 / 479001600.0;
-  p = fma(p, r, 1.0 / 39916800.0);
-  p = fma(p, r, 1.0 / 3628800.0);
-  p = fma(p, r, 1.0 / 362880.0);
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
-  p = fma(p, r, 1.0 / 720.0);
-  p = fma(p, r, 1.0 / 120.0);
+  double r = fma(nf, -0.6931471805599453 / 64.0, z);  // ln 2 as a sum of two doubles
+  r = fma(nf, -2.3190468138462996e-17 / 64.0, r);
+  double p = 1.0 / 120.0;
   p = fma(p, r, 1.0 / 24.0);
   p = fma(p, r, 1.0 / 6.0);
   p = fma(p, r, 0.5);
   p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  const double e = __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
+  p = fma(p, r, 1.0) * table[n & 63];
+  const double e = __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p));
   return z < -700.0 ? 0.0 : e;
 }
 __device__ __forceinline__ double warp_sum_d(double v) {
@@ -128,38 +124,44 @@ struct Sampler {
   float kx;
   int ki;
 
-  __device__ __forceinline__ float& at(int i) { return xs[i + (i >> 5)]; }
-  __device__ __forceinline__ double weight(float x) const { return sa_exp(((double)x - (double)M) * inv_t); }
+  // element i of the CTA is element i mod ept of a thread; position of its group of four
+  __device__ __forceinline__ int group_at(int t, int c) const {
+    const int groups = 1 << (p.ept_log2 - 2);
+    return t * groups + ((c + t) & (groups - 1));
+  }
+  __device__ __forceinline__ float& at(int i) {
+    const int t = i >> p.ept_log2, e = i & ((1 << p.ept_log2) - 1);
+    return xs[4 * group_at(t, e >> 2) + (e & 3)];
+  }
+  __device__ __forceinline__ float4 four(int t, int c) const { return reinterpret_cast<const float4*>(xs)[group_at(t, c)]; }
+  __device__ __forceinline__ double weight(float x) const { return sa_exp(((double)x - (double)M) * inv_t, sh.exp2); }
   __device__ __forceinline__ bool kept(float x, int i) const { return x > kx || (x == kx && i <= ki); }
 
+  // f(logit, index) for this thread's elements, in the order of the indices within a round; those that only fill up the
+  // thread's share are -infinity
   template <typename F>
   __device__ __forceinline__ void each(F f) {
     for (int r = 0; r < p.rounds; ++r) {
-      const int i0 = r * SA_ROUND + tid * p.ept, i1 = min(n, i0 + p.ept);
-      // four values are read before the first is used
-      for (int i = i0; i < i1; i += 4) {
-        float v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = i + k < i1 ? at(i + k) : -INFINITY;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) f(v[k], base + i + k);
+      const int t = r * SA_THREADS + tid;
+      for (int c = 0; c < 1 << (p.ept_log2 - 2); ++c) {
+        const float4 v = four(t, c);
+        const int i = base + (t << p.ept_log2) + 4 * c;
+        f(v.x, i), f(v.y, i + 1), f(v.z, i + 2), f(v.w, i + 3);
       }
     }
   }
-
   // f(logit, index, weight) for the elements that `want` takes: first which they are, then their weights, two at a time,
   // so that a warp computes as many as its busiest lane has, not one for every element that some lane has
   template <typename P, typename F>
   __device__ __forceinline__ void each_weight(P want, F f) {
     for (int r = 0; r < p.rounds; ++r) {
-      const int i0 = r * SA_ROUND + tid * p.ept, c = min(n - i0, p.ept);
+      const int t = r * SA_THREADS + tid, i0 = t << p.ept_log2;
       unsigned mask = 0;
-      for (int i = 0; i < c; i += 4) {
-        float v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = i + k < c ? at(i0 + i + k) : -INFINITY;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mask |= (unsigned)want(v[k], base + i0 + i + k) << (i + k);
+      for (int c = 0; c < 1 << (p.ept_log2 - 2); ++c) {
+        const float4 v = four(t, c);
+        const int i = base + i0 + 4 * c;
+        mask |= ((unsigned)want(v.x, i) | (unsigned)want(v.y, i + 1) << 1 | (unsigned)want(v.z, i + 2) << 2 |
+                 (unsigned)want(v.w, i + 3) << 3) << (4 * c);
       }
       while (mask) {
         const int a = __ffs(mask) - 1;
@@ -255,7 +257,7 @@ struct Sampler {
     for (int r = 0; r < rank; ++r) pre += cl.map_shared_rank(&sh.x[xb], r)->n[0];
     int k = m - pre - before - excl;
     if (k >= 0 && k < mine) {
-      const int i0 = round * SA_ROUND + tid * p.ept, i1 = min(n, i0 + p.ept);
+      const int i0 = (round * SA_THREADS + tid) << p.ept_log2, i1 = i0 + (1 << p.ept_log2);
       for (int i = i0; i < i1; ++i)
         if (kept(at(i), base + i) && at(i) == x && k-- == 0) sh.pick_i = base + i;
     }
@@ -290,7 +292,7 @@ struct Sampler {
     xb ^= 1;
     if (k >= 0 && k < all) {
       for (int r = 0; r < p.rounds; ++r) {
-        const int i0 = r * SA_ROUND + tid * p.ept, i1 = min(n, i0 + p.ept);
+        const int i0 = (r * SA_THREADS + tid) << p.ept_log2, i1 = i0 + (1 << p.ept_log2);
         int c = 0;
         for (int i = i0; i < i1; ++i) c += kept(at(i), base + i) && at(i) == x;
         int inc = c;
@@ -346,8 +348,8 @@ struct Sampler {
       double v0 = (double)h0, v1 = (double)h1;
       if (by_weight) {
         // relative to the weight at hi
-        v0 *= sa_exp((double)(2 * tid * width) * -inv_t);
-        v1 *= sa_exp((double)((2 * tid + 1) * width) * -inv_t);
+        v0 *= sa_exp((double)(2 * tid * width) * -inv_t, sh.exp2);
+        v1 *= sa_exp((double)((2 * tid + 1) * width) * -inv_t, sh.exp2);
       }
       double total, pre = block_scan(v0 + v1, total) - (v0 + v1);   // what lies before this thread's bins
       // the histogram counts weights in units of 2^-14 of the weight at hi
@@ -550,15 +552,17 @@ struct Sampler {
     __syncthreads();
     const int b = sh.pick;
     if (b >= SA_BINS) return false;      // fewer threads with logits than k
+    // a border a little below the bin's far edge, whatever the rounding: more elements on the list do no harm
+    const float border = fmaxf(low, (top - ((float)(b + 1) * 1.0001f) / scale) / half);
     each([&](float x, int i) {
-      if (x > -INFINITY && bin_of(x) <= b) {
+      if (x >= border) {
         const unsigned slot = atomicAdd(&sh.ln, 1u);
         if (slot < SA_LIST) sh.lx[slot] = x, sh.li[slot] = i;
       }
     });
     cl.sync();
     const int n_all = __reduce_add_sync(0xffffffffu, lane < size ? (int)*cl.map_shared_rank(&sh.ln, lane) : 0);
-    if (n_all > SA_LIST) {
+    if (n_all > SA_LIST || n_all < k) {
       cl.sync();                         // the lists are written anew
       return false;
     }
@@ -594,8 +598,15 @@ struct Sampler {
   __device__ void run(int row) {
     const T* x = reinterpret_cast<const T*>(p.logits) + (int64_t)row * p.sb;
     xb = 0;
-    base = rank * p.slice;
+    // The CTA's elements begin on 16 bytes: the row is led in by up to 7 that do not exist (unless the last CTA has no
+    // room for them; then it is read one by one).
+    constexpr int VL = 16 / (int)sizeof(T);
+    int lead = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+    const bool vec = lead == 0 || p.V + lead <= p.slice * size;
+    if (!vec) lead = 0;
+    base = rank * p.slice - lead;
     n = max(0, min(p.V - base, p.slice));
+    if (tid < 64) sh.exp2[tid] = exp2((double)tid / 64.0);
     const float temperature = p.temperature ? p.temperature[row] : p.temperature0;
     const float top_p = p.top_p ? p.top_p[row] : p.top_p0;
     const float min_p = p.min_p ? p.min_p[row] : p.min_p0;
@@ -603,35 +614,47 @@ struct Sampler {
     // ---- the row, once ------------------------------------------------------------------------------------------
     float mn = INFINITY, mx = -INFINITY;
     int fin = 0;
-    auto take = [&](int i, float v) {
-      at(i) = v;
+    auto look = [&](float v) -> float {
       mx = fmaxf(mx, v);
       if (v > -INFINITY) {
         ++fin;
         mn = fminf(mn, v);
       }
+      return v;
     };
-    // 16-byte loads behind the first aligned element, single ones before and after
-    constexpr int VL = 16 / (int)sizeof(T);
-    const T* src = x + base;
-    const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(T)));
-    const int nv = (n - head) / VL;
-    if (tid < head) take(tid, sa_value<T>(src[tid]));
-    for (int i = head + nv * VL + tid; i < n; i += SA_THREADS) take(i, sa_value<T>(src[i]));
-    const uint4* vec = reinterpret_cast<const uint4*>(src + head);
-    constexpr int U = 4;               // loads in flight per thread
-    for (int v0 = tid; v0 < nv; v0 += U * SA_THREADS) {
-      uint4 raw[U];
+    const int held = p.rounds * (SA_THREADS << p.ept_log2);
+    if (vec) {
+      constexpr int U = 4;             // loads in flight per thread
+      const T* src = x + base;
+      for (int v0 = tid; v0 * VL < held; v0 += U * SA_THREADS) {
+        uint4 raw[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (v0 + u * SA_THREADS < nv) raw[u] = __ldg(vec + v0 + u * SA_THREADS);
+        for (int u = 0; u < U; ++u) {
+          const int i = (v0 + u * SA_THREADS) * VL;
+          raw[u] = make_uint4(0, 0, 0, 0);
+          if (base + i >= 0 && i + VL <= n) raw[u] = __ldg(reinterpret_cast<const uint4*>(src + i));
+        }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (v0 + u * SA_THREADS >= nv) break;
-        const T* e = reinterpret_cast<const T*>(&raw[u]);
+        for (int u = 0; u < U; ++u) {
+          const int i = (v0 + u * SA_THREADS) * VL;
+          if (i >= held) break;
+          const bool whole = base + i >= 0 && i + VL <= n;
+          const T* e = reinterpret_cast<const T*>(&raw[u]);
+          float v[VL];
 #pragma unroll
-        for (int j = 0; j < VL; ++j) take(head + (v0 + u * SA_THREADS) * VL + j, sa_value<T>(e[j]));
+          for (int j = 0; j < VL; ++j) {
+            if (whole) v[j] = sa_value<T>(e[j]);
+            else v[j] = base + i + j >= 0 && i + j < n ? sa_value<T>(src[i + j]) : -INFINITY;
+            look(v[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < VL; j += 4)
+            reinterpret_cast<float4*>(xs)[group_at((i + j) >> p.ept_log2, ((i + j) & ((1 << p.ept_log2) - 1)) >> 2)] =
+                make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        }
       }
+    } else {
+      for (int i = tid; i < held; i += SA_THREADS) at(i) = i < n ? look(sa_value<T>(x[base + i])) : -INFINITY;
     }
     SaXchg o;
     exchange(0.0, 0.0, mn, mx, fin, 0, o);
@@ -650,7 +673,7 @@ struct Sampler {
     if (M == INFINITY) {
       // the limit of ever larger logits: those at +infinity share the probability
       int c = 0;
-      for (int i = tid; i < n; i += SA_THREADS) {
+      for (int i = tid; i < held; i += SA_THREADS) {
         const float v = at(i) == INFINITY ? 0.f : -INFINITY;
         at(i) = v;
         c += v == 0.f;
@@ -696,7 +719,8 @@ struct Sampler {
     double mine[SA_MAX_ROUNDS] = {0.0, 0.0, 0.0}, s = 0.0;
     each_weight([&](float v, int i) { return kept(v, i); },
                 [&](float v, int i, double w) {
-                  const int r = (i - base) / SA_ROUND;
+                  const int r = (i - base) >> (p.ept_log2 + 9);
+                  static_assert(SA_THREADS == 512, "2^9 threads");
                   if (w >= min_p || v == M) {
 #pragma unroll
                     for (int x = 0; x < SA_MAX_ROUNDS; ++x) mine[x] += x == r ? w : 0.0;
@@ -790,18 +814,22 @@ struct Sampler {
       __syncthreads();
       for (int w = 0; w < SA_WARPS; ++w) before += sh.red_d[0][w];
     }
-    if (tid == 0) {
-      const int i0 = kr * SA_ROUND + kt * p.ept, i1 = min(n, i0 + p.ept);
-      double run_sum = before, wt = 0.0;
-      int token = -1;
-      for (int i = i0; i < i1; ++i) {
-        const double w = mass(i);
-        if (w > 0.0) token = base + i, wt = w;
-        run_sum += w;
-        if (w > 0.0 && run_sum > goal) break;
+    if (warp == 0) {
+      // an element per lane
+      const int i0 = (kr * SA_THREADS + kt) << p.ept_log2;
+      const double w = lane < (1 << p.ept_log2) ? mass(i0 + lane) : 0.0;
+      double inc = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double v = shfl_up_d(inc, o);
+        if (lane >= o) inc += v;
       }
-      p.token[row] = token;
-      if (p.logprob) p.logprob[row] = (float)log(wt / W);
+      const unsigned passed = __ballot_sync(0xffffffffu, w > 0.0 && before + inc > goal);
+      const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
+      if (lane == (passed ? __ffs(passed) - 1 : 31 - __clz(any))) {
+        p.token[row] = base + i0 + lane;
+        if (p.logprob) p.logprob[row] = (float)log(w / W);
+      }
     }
   }
 };
@@ -820,9 +848,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleParam
 
 template <typename T>
 static int sample_launch(const SampleParams& prm, int B, int cluster, cudaStream_t st) {
-  const int smem = prm.rounds * SA_THREADS * (SA_EPT + 1) * 4;
+  const int smem = prm.rounds * (SA_THREADS << prm.ept_log2) * 4;
   cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       SA_MAX_ROUNDS * SA_THREADS * (SA_EPT + 1) * 4);
+                                       SA_MAX_ROUNDS * SA_ROUND * 4);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(sample)");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(B * cluster);
@@ -864,9 +892,15 @@ extern "C" int fa_sample(const void* logits, int dtype, int B, int V, int64_t lo
   prm.logits = logits;
   prm.sb = logits_sb;
   prm.V = V;
-  prm.slice = ceil_div(V, cluster);
+  // room for the elements that lead a row in, as long as it is there
+  const int lead = 16 / (dtype == FA_DTYPE_F32 ? 4 : 2) - 1;
+  prm.slice = ceil_div(ceil_div(V + lead, cluster), 8) * 8;
+  if (prm.slice > SA_MAX_ROUNDS * SA_ROUND || (prm.slice > SA_ROUND && ceil_div(V, cluster) <= SA_ROUND))
+    prm.slice = ceil_div(ceil_div(V, cluster), 8) * 8;
   prm.rounds = ceil_div(prm.slice, SA_ROUND);
-  prm.ept = prm.rounds > 1 ? SA_EPT : ceil_div(prm.slice, SA_THREADS);
+  prm.ept_log2 = 2;
+  while (prm.rounds == 1 && (SA_THREADS << prm.ept_log2) < prm.slice) ++prm.ept_log2;
+  if (prm.rounds > 1) prm.ept_log2 = 5;
   prm.u = u;
   prm.temperature = temperature, prm.temperature0 = temperature0;
   prm.top_k = top_k, prm.top_k0 = top_k0;
