@@ -4,6 +4,7 @@ There is no fallback: if the library has not been built, importing this module r
 """
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libfourier_b200.so")
@@ -98,6 +99,16 @@ class PagedAttnArgs(C.Structure):
     ]
 
 
+def packer(cls):
+    """A ``struct.Struct`` with the layout of an argument block: packing all fields at once takes a tenth of the time of
+    setting them one by one, and the small calls of a decode step are bound by their host side."""
+    codes = {i32: "i", i64: "q", vp: "P", f32: "f", sz: "N"}
+    return struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_))
+
+
+pack_rope, pack_paged_attn, pack_scratch = packer(RopeArgs).pack, packer(PagedAttnArgs).pack, struct.Struct("@PN").pack
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise RuntimeError(
@@ -142,11 +153,12 @@ def _load():
     lib.fa_layer_scratch_bytes.restype = sz
     lib.fa_layer_attend.argtypes = [vp, i32, i32, i32, vp, i64, f32, vp, vp, vp, vp, sz, vp, vp]
     lib.fa_layer_decode_path.argtypes = [vp]
-    lib.fa_qk_norm_rope.argtypes = [C.POINTER(RopeArgs), vp]
-    lib.fa_paged_append.argtypes = [C.POINTER(RopeArgs), vp]
-    lib.fa_paged_attn_scratch_bytes.argtypes = [C.POINTER(PagedAttnArgs)]
+    # the argument blocks are passed as packed bytes
+    lib.fa_qk_norm_rope.argtypes = [C.c_char_p, vp]
+    lib.fa_paged_append.argtypes = [C.c_char_p, vp]
+    lib.fa_paged_attn_scratch_bytes.argtypes = [C.c_char_p]
     lib.fa_paged_attn_scratch_bytes.restype = sz
-    lib.fa_paged_attn.argtypes = [C.POINTER(PagedAttnArgs), vp]
+    lib.fa_paged_attn.argtypes = [C.c_char_p, vp]
     lib.fa_sample.argtypes = [vp, C.c_int, C.c_int, C.c_int, i64, vp, vp, f32, vp, C.c_int, vp, f32, vp, f32, vp, vp, vp]
     for name in EXPORTS:
         f = getattr(lib, name)

@@ -8,6 +8,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "fourier_b200.h"
 
 namespace fa {
@@ -109,6 +111,19 @@ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int sm_count();
+
+// Raises a kernel's limit of dynamic shared memory, once per device.
+template <auto Kernel>
+inline int allow_smem(int bytes, const char* what) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < 64 && ((done.load(std::memory_order_relaxed) >> dev) & 1)) return FA_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return FA_OK;
+}
 
 // (cols x rows x B) tiled tensor map of a 16-bit tensor, 128-byte swizzle, out-of-range elements read as 0.
 // box_cols * 2 bytes must not exceed 128.  Strides in elements.

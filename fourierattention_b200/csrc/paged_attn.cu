@@ -487,8 +487,8 @@ static PaPlan pa_plan(const fa_paged_attn_args_t* a) {
 template <typename T, int D, int NT>
 static int pa_stream_launch(const PaStreamParams& prm, cudaStream_t st) {
   constexpr int smem = PaStream<D>::SMEM;
-  cudaError_t e = cudaFuncSetAttribute(paged_stream_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_stream)");
+  const int rc = allow_smem<paged_stream_kernel<T, D, NT>>(smem, "cudaFuncSetAttribute(paged_stream)");
+  if (rc != FA_OK) return rc;
   paged_stream_kernel<T, D, NT><<<prm.p.ctas, 256, smem, st>>>(prm);
   FA_CHECK_LAUNCH("fa_paged_attn");
   return FA_OK;
@@ -497,8 +497,8 @@ static int pa_stream_launch(const PaStreamParams& prm, cudaStream_t st) {
 template <typename T, int D>
 static int pa_tile_launch(const PaTileParams& prm, cudaStream_t st) {
   constexpr int smem = PaTile<D>::SMEM;
-  cudaError_t e = cudaFuncSetAttribute(paged_tile_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_tile)");
+  const int rc = allow_smem<paged_tile_kernel<T, D>>(smem, "cudaFuncSetAttribute(paged_tile)");
+  if (rc != FA_OK) return rc;
   paged_tile_kernel<T, D><<<prm.p.ctas, PT_THREADS, smem, st>>>(prm);
   FA_CHECK_LAUNCH("fa_paged_attn(tile)");
   return FA_OK;

@@ -849,9 +849,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleParam
 template <typename T>
 static int sample_launch(const SampleParams& prm, int B, int cluster, cudaStream_t st) {
   const int smem = prm.rounds * (SA_THREADS << prm.ept_log2) * 4;
-  cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       SA_MAX_ROUNDS * SA_ROUND * 4);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(sample)");
+  const int rc = allow_smem<sample_kernel<T>>(SA_MAX_ROUNDS * SA_ROUND * 4, "cudaFuncSetAttribute(sample)");
+  if (rc != FA_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(B * cluster);
   cfg.blockDim = dim3(SA_THREADS);
@@ -863,7 +862,7 @@ static int sample_launch(const SampleParams& prm, int B, int cluster, cudaStream
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, prm);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, prm);
   if (e != cudaSuccess) return cuda_fail(e, "fa_sample");
   return FA_OK;
 }

@@ -459,13 +459,16 @@ def merge(o, m, l):
 
 # ---- a served batch outside the compressed span: norm + rotation, paged cache, shared prefix, sampling ------------------
 
-def _on(dev, *ts):
-    """Every given tensor on ``dev``, a CUDA device."""
-    if dev.type != "cuda":
+_raw_stream, _device_index = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+def _on(index, *ts):
+    """Every given tensor on CUDA device ``index`` (-1: a CPU tensor, which is refused)."""
+    if index < 0:
         raise RuntimeError("fourierattention_b200 kernels need CUDA tensors (there is no CPU path)")
     for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on different devices: {t.device} and {dev}")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"tensors on different devices: {t.device} and cuda:{index}")
 
 
 def _no_grad(*ts):
@@ -475,71 +478,74 @@ def _no_grad(*ts):
                 raise RuntimeError("this operator has no backward pass: call it under torch.no_grad()")
 
 
-def _heads3(t, name, dtype=None):
-    """Sizes of a (tokens, heads, D) tensor with a contiguous last dimension."""
-    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+def _heads3(t, name, dtype):
+    """Shape and strides of a (tokens, heads, D) tensor with a contiguous last dimension."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or (stride[2] != 1 and shape[2] > 1):
         raise ValueError(f"{name}: expected (tokens, heads, head_dim) with a contiguous last dimension")
-    if dtype is not None and t.dtype != dtype:
+    if t.dtype != dtype:
         raise ValueError(f"{name}: expected dtype {dtype}, got {t.dtype}")
-    return t.shape
+    return shape, stride
 
 
 def _int32(t, name, shape):
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or (t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1):
+    if t.dtype != torch.int32 or t.shape != shape or (t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1):
         raise ValueError(f"{name}: expected int32 {shape} with a contiguous last dimension, "
                          f"got {t.dtype} {tuple(t.shape)}")
 
 
-def _call(fn, name, dev, *args):
-    """One call of the library on the current stream of ``dev``."""
-    index = dev.index
-    if torch.cuda.current_device() == index:
-        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+def _call(fn, name, index, *args):
+    """One call of the library on the current stream of device ``index``."""
+    if _device_index() == index:
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+            rc = fn(*args, _raw_stream(index))
     if rc:
         check(rc, name)
 
 
-def _rope_args(a, q, k, inv_freq, q_weight, k_weight, eps, q_out):
-    """The part of the argument block that qk_norm_rope and paged_append share; returns the query output."""
-    ref = q if q is not None else k
-    a.dtype = _dt(ref)
-    tokens, heads, D = _heads3(ref, "q" if q is not None else "k")
-    a.tokens, a.D = tokens, D
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
-        raise ValueError("inv_freq: expected a contiguous float32 vector")
-    a.R, a.inv_freq = 2 * inv_freq.shape[0], inv_freq.data_ptr()
-    if k is not None:
-        if k is not ref and _heads3(k, "k", ref.dtype)[::2] != (tokens, D):
-            raise ValueError("q and k must have the same tokens and head dimension")
-        a.Hkv, a.k, a.k_st, a.k_sh = k.shape[1], k.data_ptr(), k.stride(0), k.stride(1)
-    if q is not None:
-        if q_out is None:
-            q_out = torch.empty((tokens, heads, D), dtype=q.dtype, device=q.device)
-        elif _heads3(q_out, "q_out", q.dtype) != q.shape:
-            raise ValueError("q_out must have the shape of q")
-        a.Hq, a.q, a.q_st, a.q_sh = heads, q.data_ptr(), q.stride(0), q.stride(1)
-        a.q_out, a.qo_st, a.qo_sh = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+def _like(out, name, shape, dtype):
+    """A given output has the shape of its input."""
+    if out is not None and _heads3(out, name, dtype)[0] != shape:
+        raise ValueError(f"{name} must have the shape of its input")
+
+
+def _out3(out, like, shape):
+    """The output tensor (a new one if not given) and its strides."""
+    if out is None:
+        return like.new_empty(shape), (shape[1] * shape[2], shape[2])
+    return out, out.stride()
+
+
+def _norm_weights(q_weight, k_weight, D, dtype):
+    """(w_f32, pointers) of the norm weights."""
+    if q_weight is None and k_weight is None:
+        return 0, 0, 0
+    f32 = None
     for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is None:
             continue
-        if tuple(w.shape) != (D,) or not w.is_contiguous() or w.dtype not in (ref.dtype, torch.float32):
-            raise ValueError(f"{name}: expected a contiguous ({D},) tensor of {ref.dtype} or float32")
-        if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        if w.shape != (D,) or not w.is_contiguous() or (w.dtype != dtype and w.dtype != torch.float32):
+            raise ValueError(f"{name}: expected a contiguous ({D},) tensor of {dtype} or float32")
+        if f32 is not None and f32 != (w.dtype == torch.float32):
             raise ValueError("q_weight and k_weight must share their dtype")
-        a.w_f32 = 1 if w.dtype == torch.float32 else 0
-        setattr(a, name, w.data_ptr())
-    a.eps = eps
-    return q_out
+        f32 = w.dtype == torch.float32
+    return (1 if f32 else 0, q_weight.data_ptr() if q_weight is not None else 0,
+            k_weight.data_ptr() if k_weight is not None else 0)
 
 
-def _positions(a, positions, tokens):
-    if positions.dtype not in (torch.int64, torch.int32) or tuple(positions.shape) != (tokens,) \
-            or not positions.is_contiguous():
+def _rotary_width(inv_freq):
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq: expected a contiguous float32 vector")
+    return 2 * inv_freq.shape[0]
+
+
+def _positions64(positions, tokens):
+    """1 for int64 positions, 0 for int32."""
+    if positions.dtype not in (torch.int64, torch.int32) or positions.shape != (tokens,) or not positions.is_contiguous():
         raise ValueError(f"positions: expected a contiguous int64 or int32 ({tokens},) tensor")
-    a.positions, a.pos_i64 = positions.data_ptr(), 1 if positions.dtype == torch.int64 else 0
+    return 1 if positions.dtype == torch.int64 else 0
 
 
 def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, q_out=None, k_out=None):
@@ -550,34 +556,41 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e
     arithmetic with exact angles, one rounding.  Returns (q, k), written to ``q_out`` / ``k_out`` if given (the inputs
     themselves are allowed)."""
     _no_grad(q, k, q_weight, k_weight)
-    a = _lib.RopeArgs()
-    _heads3(q, "q")
-    q_out = _rope_args(a, q, k, inv_freq, q_weight, k_weight, eps, q_out)
-    _positions(a, positions, q.shape[0])
-    if k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    elif _heads3(k_out, "k_out", k.dtype) != k.shape:
-        raise ValueError("k_out must have the shape of k")
-    a.k_out, a.ko_st, a.ko_sh = k_out.data_ptr(), k_out.stride(0), k_out.stride(1)
-    _on(q.device, k, positions, inv_freq, q_weight, k_weight, q_out, k_out)
-    _call(lib.fa_qk_norm_rope, "fa_qk_norm_rope", q.device, C.byref(a))
+    code, dtype = _dt(q), q.dtype
+    qs, qst = _heads3(q, "q", dtype)
+    ks, kst = _heads3(k, "k", dtype)
+    tokens, Hq, D = qs
+    if ks[0] != tokens or ks[2] != D:
+        raise ValueError("q and k must have the same tokens and head dimension")
+    R, wide = _rotary_width(inv_freq), _positions64(positions, tokens)
+    w_f32, qw, kw = _norm_weights(q_weight, k_weight, D, dtype)
+    _like(q_out, "q_out", qs, dtype)
+    _like(k_out, "k_out", ks, dtype)
+    index = q.get_device()
+    _on(index, k, positions, inv_freq, q_weight, k_weight, q_out, k_out)
+    q_out, qost = _out3(q_out, q, qs)
+    k_out, kost = _out3(k_out, k, ks)
+    a = _lib.pack_rope(tokens, Hq, ks[1], D, R, code, w_f32, wide, q.data_ptr(), k.data_ptr(), 0, qst[0], qst[1], kst[0],
+                       kst[1], 0, 0, q_out.data_ptr(), k_out.data_ptr(), qost[0], qost[1], kost[0], kost[1],
+                       positions.data_ptr(), inv_freq.data_ptr(), qw, kw, eps, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                       0, 0)
+    _call(lib.fa_qk_norm_rope, "fa_qk_norm_rope", index, a)
     _count(1)
     return q_out, k_out
 
 
-def _pages(a, k_pages, v_pages, dtype, Hkv, D):
-    """Sizes and strides of a cache of pages (num_pages, Hkv, page_size, D)."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != dtype or v_pages.dtype != dtype \
-            or k_pages.shape[1] != Hkv or k_pages.shape[3] != D or k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+def _pages(k_pages, v_pages, dtype, Hkv, D):
+    """Shape and strides of a cache of pages (num_pages, Hkv, page_size, D)."""
+    shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
+    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype != dtype or v_pages.dtype != dtype \
+            or shape[1] != Hkv or shape[3] != D or ks[3] != 1 or vs[3] != 1:
         raise ValueError(f"k_pages, v_pages: expected {dtype} (num_pages, {Hkv}, page_size, {D}) with a contiguous last "
                          "dimension")
-    a.num_pages, a.page_size = k_pages.shape[0], k_pages.shape[2]
-    a.k_pages, a.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
-    a.kp_sp, a.kp_sh, a.kp_sr, _ = k_pages.stride()
-    a.vp_sp, a.vp_sh, a.vp_sr, _ = v_pages.stride()
+    return shape, ks, vs
 
 
-def _sequences(a, page_table, kv_lens, cu_seqlens, tokens):
+def _sequences(page_table, kv_lens, cu_seqlens, tokens):
+    """Shape of the page table."""
     if page_table.dim() != 2:
         raise ValueError("page_table: expected int32 (sequences, pages)")
     B, most = page_table.shape
@@ -585,11 +598,9 @@ def _sequences(a, page_table, kv_lens, cu_seqlens, tokens):
     _int32(kv_lens, "kv_lens", (B,))
     if cu_seqlens is not None:
         _int32(cu_seqlens, "cu_seqlens", (B + 1,))
-        a.cu_seqlens = cu_seqlens.data_ptr()
     elif tokens != B:
         raise ValueError(f"{tokens} tokens of {B} sequences: without cu_seqlens there is one token per sequence")
-    a.B, a.max_pages = B, most
-    a.page_table, a.table_sb, a.kv_lens = page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr()
+    return B, most
 
 
 def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, inv_freq, cu_seqlens=None, positions=None, pos_offset=0,
@@ -602,20 +613,36 @@ def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, inv_freq, cu_seqle
     last sequence, indices outside the table and page ids that name no page write nothing.  Returns the rotated
     queries (``q_out`` if given; None without q)."""
     _no_grad(k, v, q, q_weight, k_weight)
-    a = _lib.RopeArgs()
-    tokens, Hkv, D = _heads3(k, "k")
-    if _heads3(v, "v", k.dtype) != k.shape:
+    code, dtype = _dt(k), k.dtype
+    ks, kst = _heads3(k, "k", dtype)
+    vs, vst = _heads3(v, "v", dtype)
+    if vs != ks:
         raise ValueError("k and v must have the same shape")
-    q_out = _rope_args(a, q, k, inv_freq, q_weight, k_weight, eps, q_out)
-    a.v, a.v_st, a.v_sh = v.data_ptr(), v.stride(0), v.stride(1)
-    _pages(a, k_pages, v_pages, k.dtype, Hkv, D)
-    _sequences(a, page_table, kv_lens, cu_seqlens, tokens)
+    tokens, Hkv, D = ks
+    R = _rotary_width(inv_freq)
+    w_f32, qw, kw = _norm_weights(q_weight, k_weight, D, dtype)
+    pages, kp, vp = _pages(k_pages, v_pages, dtype, Hkv, D)
+    B, most = _sequences(page_table, kv_lens, cu_seqlens, tokens)
+    Hq, q_ptr, qo_ptr, qst, qost = 0, 0, 0, (0, 0), (0, 0)
+    if q is not None:
+        qs, qst = _heads3(q, "q", dtype)
+        if qs[0] != tokens or qs[2] != D:
+            raise ValueError("q and k must have the same tokens and head dimension")
+        _like(q_out, "q_out", qs, dtype)
+    pos_ptr, wide = 0, 0
     if positions is not None:
-        _positions(a, positions, tokens)
-    a.pos_offset = pos_offset
-    _on(k.device, v, q, q_out, k_pages, v_pages, page_table, kv_lens, cu_seqlens, positions, inv_freq, q_weight,
-        k_weight)
-    _call(lib.fa_paged_append, "fa_paged_append", k.device, C.byref(a))
+        wide, pos_ptr = _positions64(positions, tokens), positions.data_ptr()
+    index = k.get_device()
+    _on(index, v, q, q_out, k_pages, v_pages, page_table, kv_lens, cu_seqlens, positions, inv_freq, q_weight, k_weight)
+    if q is not None:
+        q_out, qost = _out3(q_out, q, qs)
+        Hq, q_ptr, qo_ptr = qs[1], q.data_ptr(), q_out.data_ptr()
+    a = _lib.pack_rope(tokens, Hq, Hkv, D, R, code, w_f32, wide, q_ptr, k.data_ptr(), v.data_ptr(), qst[0], qst[1], kst[0],
+                       kst[1], vst[0], vst[1], qo_ptr, 0, qost[0], qost[1], 0, 0, pos_ptr, inv_freq.data_ptr(), qw, kw, eps,
+                       B, pages[2], most, pages[0], k_pages.data_ptr(), v_pages.data_ptr(), kp[0], kp[1], kp[2], vp[0],
+                       vp[1], vp[2], page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(),
+                       cu_seqlens.data_ptr() if cu_seqlens is not None else 0, pos_offset)
+    _call(lib.fa_paged_append, "fa_paged_append", index, a)
     _count(1)
     return q_out
 
@@ -630,57 +657,56 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens=None, p
     -infinity; tokens behind the last sequence are left as they were.  Scratch comes from PyTorch's allocator, per
     call."""
     _no_grad(q, k_pages, v_pages)
-    a = _lib.PagedAttnArgs()
-    a.dtype = _dt(q)
-    tokens, Hq, D = _heads3(q, "q")
+    code, dtype = _dt(q), q.dtype
+    qs, qst = _heads3(q, "q", dtype)
+    tokens, Hq, D = qs
     if k_pages.dim() != 4:
         raise ValueError("k_pages: expected (num_pages, kv_heads, page_size, head_dim)")
-    Hkv = k_pages.shape[1]
-    a.tokens, a.Hq, a.Hkv, a.D = tokens, Hq, Hkv, D
-    _pages(a, k_pages, v_pages, q.dtype, Hkv, D)
-    _sequences(a, page_table, kv_lens, cu_seqlens, tokens)
+    pages, kp, vp = _pages(k_pages, v_pages, dtype, k_pages.shape[1], D)
+    B, most = _sequences(page_table, kv_lens, cu_seqlens, tokens)
+    pre_ptr, n_pre = 0, 0
     if prefix_len:
         if prefix_pages is None or prefix_pages.dim() != 1:
             raise ValueError("prefix_pages: expected an int32 vector of page ids")
-        _int32(prefix_pages, "prefix_pages", (prefix_pages.shape[0],))
-        a.prefix_pages, a.n_prefix_pages, a.prefix_len = prefix_pages.data_ptr(), prefix_pages.shape[0], prefix_len
-    a.sm_scale = -1.0 if sm_scale is None else sm_scale
-    if out is None:
-        out = torch.empty((tokens, Hq, D), dtype=q.dtype, device=q.device)
-    elif _heads3(out, "out", q.dtype) != q.shape:
-        raise ValueError("out must have the shape of q")
-    lse = torch.empty((tokens, Hq), dtype=torch.float32, device=q.device) if return_lse else None
-    a.q, a.q_st, a.q_sh = q.data_ptr(), q.stride(0), q.stride(1)
-    a.out, a.o_st, a.o_sh = out.data_ptr(), out.stride(0), out.stride(1)
-    a.lse = lse.data_ptr() if return_lse else None
-    _on(q.device, k_pages, v_pages, page_table, kv_lens, cu_seqlens, prefix_pages if prefix_len else None, out)
-    if tokens:
-        index = q.device.index
-        if torch.cuda.current_device() != index:
-            with torch.cuda.device(index):
-                return _paged_attention(a, q.device, out, lse, prefix_len)
-        return _paged_attention(a, q.device, out, lse, prefix_len)
-    return (out, lse) if return_lse else out
-
-
-def _paged_attention(a, dev, out, lse, prefix_len):
-    nbytes = lib.fa_paged_attn_scratch_bytes(C.byref(a))
-    if nbytes:
-        # of this call alone: a buffer kept between calls would be shared by captured graphs
-        sc = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        a.scratch, a.scratch_bytes = sc.data_ptr(), nbytes
-    rc = lib.fa_paged_attn(C.byref(a), torch.cuda.current_stream(dev).cuda_stream)
+        n_pre = prefix_pages.shape[0]
+        _int32(prefix_pages, "prefix_pages", (n_pre,))
+        pre_ptr = prefix_pages.data_ptr()
+    _like(out, "out", qs, dtype)
+    index = q.get_device()
+    _on(index, k_pages, v_pages, page_table, kv_lens, cu_seqlens, prefix_pages if prefix_len else None, out)
+    out, ost = _out3(out, q, qs)
+    lse = q.new_empty((tokens, Hq), dtype=torch.float32) if return_lse else None
+    block = bytearray(_lib.pack_paged_attn(
+        tokens, B, Hq, pages[1], D, pages[2], pages[0], most, n_pre, prefix_len, code,
+        -1.0 if sm_scale is None else sm_scale, q.data_ptr(), qst[0], qst[1], out.data_ptr(), ost[0], ost[1],
+        lse.data_ptr() if return_lse else 0, k_pages.data_ptr(), v_pages.data_ptr(), kp[0], kp[1], kp[2], vp[0], vp[1],
+        vp[2], page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(),
+        cu_seqlens.data_ptr() if cu_seqlens is not None else 0, pre_ptr, 0, 0))
+    if _device_index() == index:
+        rc = _paged_attention(block, q, index)
+    else:
+        with torch.cuda.device(index):
+            rc = _paged_attention(block, q, index)
     if rc:
         check(rc, "fa_paged_attn")
     _count(3 if prefix_len else 2)
-    return out if lse is None else (out, lse)
+    return (out, lse) if return_lse else out
 
 
-def _row_parameter(value, name, dtype, B):
+def _paged_attention(block, q, index):
+    nbytes = lib.fa_paged_attn_scratch_bytes(bytes(block))
+    # of this call alone: a buffer kept between calls would be shared by captured graphs
+    sc = q.new_empty((nbytes,), dtype=torch.uint8)
+    block[-16:] = _lib.pack_scratch(sc.data_ptr(), nbytes)        # the last two fields
+    return lib.fa_paged_attn(bytes(block), _raw_stream(index))
+
+
+def _row_parameter(value, name, dtype, B, index):
     """(pointer, value) of a per-row tensor or of one number for all rows."""
     if isinstance(value, torch.Tensor):
-        if value.dtype != dtype or tuple(value.shape) != (B,) or not value.is_contiguous():
+        if value.dtype != dtype or value.shape != (B,) or not value.is_contiguous():
             raise ValueError(f"{name}: expected a number or a contiguous {dtype} ({B},) tensor")
+        _on(index, value)
         return value.data_ptr(), 0
     return None, value
 
@@ -694,22 +720,23 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_log
     float32 logarithm of the probability each had in the kept distribution.  NaN logits are never drawn; a row without a
     logit above -infinity gives token -1."""
     _no_grad(logits)
-    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise ValueError("logits: expected (B, V) with a contiguous last dimension")
-    B, V = logits.shape
-    dtype = _lib.FA_DTYPE_F32 if logits.dtype == torch.float32 else _dt(logits)
-    if u.dtype != torch.float32 or tuple(u.shape) != (B,) or not u.is_contiguous():
+    B, V = shape
+    code = _lib.FA_DTYPE_F32 if logits.dtype == torch.float32 else _dt(logits)
+    if u.dtype != torch.float32 or u.shape != (B,) or not u.is_contiguous():
         raise ValueError(f"u: expected a contiguous float32 ({B},) tensor")
-    tp, tv = _row_parameter(temperature, "temperature", torch.float32, B)
-    kp, kv = _row_parameter(top_k, "top_k", torch.int32, B)
-    pp, pv = _row_parameter(top_p, "top_p", torch.float32, B)
-    mp, mv = _row_parameter(min_p, "min_p", torch.float32, B)
-    dev = logits.device
-    _on(dev, u, *(t for t in (temperature, top_k, top_p, min_p) if isinstance(t, torch.Tensor)))
-    token = torch.empty((B,), dtype=torch.int64, device=dev)
-    logprob = torch.empty((B,), dtype=torch.float32, device=dev) if return_logprob else None
-    _call(lib.fa_sample, "fa_sample", dev, logits.data_ptr(), dtype, B, V, logits.stride(0), u.data_ptr(), tp, tv, kp, kv,
-          pp, pv, mp, mv, token.data_ptr(), logprob.data_ptr() if return_logprob else None)
+    index = u.get_device()
+    tp, tv = _row_parameter(temperature, "temperature", torch.float32, B, index)
+    kp, kv = _row_parameter(top_k, "top_k", torch.int32, B, index)
+    pp, pv = _row_parameter(top_p, "top_p", torch.float32, B, index)
+    mp, mv = _row_parameter(min_p, "min_p", torch.float32, B, index)
+    _on(index, logits)
+    token = u.new_empty((B,), dtype=torch.int64)
+    logprob = u.new_empty((B,)) if return_logprob else None
+    _call(lib.fa_sample, "fa_sample", index, logits.data_ptr(), code, B, V, stride[0], u.data_ptr(), tp, tv, kp, kv, pp, pv,
+          mp, mv, token.data_ptr(), logprob.data_ptr() if return_logprob else None)
     _count(1)
     return (token, logprob) if return_logprob else token
 

@@ -32,6 +32,11 @@ def test_argument_blocks_match_c(ops, ctype, pytype):
         subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), src, "-o", exe])
         vals = [int(x) for x in subprocess.check_output([exe]).split()]
     assert vals == [C.sizeof(mirror)] + [getattr(mirror, f).offset for f in fields]
+    # and packed at once it is the same bytes as filled in field by field
+    block, values = mirror(), list(range(3, 3 + len(fields)))
+    for name, v in zip(fields, values):
+        setattr(block, name, v)
+    assert ops._lib.packer(mirror).pack(*values) == bytes(block)
 
 
 def _t(*shape, dtype=BF):
@@ -130,7 +135,7 @@ def test_inputs_that_need_a_gradient_are_refused(ops):
 def test_library_refuses(ops):
     """The C entries check sizes, alignment and pointers themselves."""
     lib, L = ops.lib, ops._lib
-    call = lambda f, a: f(C.byref(a), None)
+    call = lambda f, a: f(bytes(a), None)
 
     def rope(**kw):
         a = L.RopeArgs()
@@ -164,8 +169,8 @@ def test_library_refuses(ops):
                    (dict(q_st=513), -4), (dict(out=4104), -4), (dict(kp_sr=68), -4), (dict(v_pages=4100), -4), (dict(scratch=None), -5),
                    (dict(scratch_bytes=16), -5), (dict(scratch=4100), -5), (dict(tokens=0, B=0), 0)):
         assert call(lib.fa_paged_attn, attn(**kw)) == rc, kw
-    assert lib.fa_paged_attn_scratch_bytes(C.byref(attn())) > 0
-    assert lib.fa_paged_attn_scratch_bytes(C.byref(attn(D=96))) == 0
+    assert lib.fa_paged_attn_scratch_bytes(bytes(attn())) > 0
+    assert lib.fa_paged_attn_scratch_bytes(bytes(attn(D=96))) == 0
     one = lambda **kw: lib.fa_sample(*{**dict(x=4096, dt=1, B=2, V=10, sb=10, u=4096, t=None, t0=1.0, k=None, k0=0, p=None, p0=1.0, m=None,
                                               m0=0.0, tok=4096, lp=None, st=None), **kw}.values())
     assert one(dt=3) == -3 and one(V=0) == -2 and one(B=-1) == -2 and one(V=393217) == -5 and one(x=None) == -1
