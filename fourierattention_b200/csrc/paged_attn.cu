@@ -87,10 +87,10 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     if (pa_smem(pa_dyn) & 1023u) sh.dead = 1;      // the swizzle pattern goes by the address
   }
+  pa_let_next_begin();
   PaUnit u;
   int t;
   const PaRange range = pa_locate<256>(c, p, blockIdx.x, sh.loc, u, t);   // (its barriers order the initialisation too)
-  if (range.beg >= range.end) return;
 
   // ---- this warp's fetches: the same walk as below, ST groups of 16 keys ahead -----------------------------------------
   PaUnit fu = u;
@@ -276,37 +276,35 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
         x += __shfl_xor_sync(0xffffffffu, x, 16);
         if (g == 0) sh.m[warp][nt * 8 + c2 + j] = m[nt][j], sh.l[warp][nt * 8 + c2 + j] = x;
       }
-    __syncthreads();
     const bool first = t == 0, last = t_end == u.tiles;
     const bool whole = first && last;
-    const float poison = sh.dead ? __int_as_float(0x7fc00000) : 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float mx = -INFINITY;
-        for (int w = 0; w < C::WARPS; ++w) mx = fmaxf(mx, sh.m[w][nt * 8 + c2 + j]);
-        const float f = m[nt][j] == -INFINITY ? 0.f : pa_ex2(m[nt][j] - mx);
         float* dst = obuf + (warp * 8 + c2 + j) * C::OPITCH + g;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
-          dst[16 * i] = o[nt][i][j] * f;
-          dst[16 * i + 8] = o[nt][i][j + 2] * f;
+          dst[16 * i] = o[nt][i][j];
+          dst[16 * i + 8] = o[nt][i][j + 2];
         }
       }
       __syncthreads();
+      const float poison = sh.dead ? __int_as_float(0x7fc00000) : 0.f;
       for (int e = tid; e < 8 * (D / 4); e += 256) {
         const int col = e / (D / 4), d4 = (e % (D / 4)) * 4;
         const int r = nt * 8 + col;
         if (r >= n_rows) continue;
         float mx = -INFINITY, lsum = 0.f;
+#pragma unroll
         for (int w = 0; w < C::WARPS; ++w) mx = fmaxf(mx, sh.m[w][r]);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < C::WARPS; ++w) {
-          if (sh.m[w][r] > -INFINITY) lsum += sh.l[w][r] * pa_ex2(sh.m[w][r] - mx);
+          const float f = sh.m[w][r] == -INFINITY ? 0.f : pa_ex2(sh.m[w][r] - mx);
+          lsum = fmaf(sh.l[w][r], f, lsum);
           const float4 v = *reinterpret_cast<const float4*>(obuf + (w * 8 + col) * C::OPITCH + d4);
-          acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+          acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y), acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
         }
         acc.x += poison, acc.y += poison, acc.z += poison, acc.w += poison;
         lsum += poison;
@@ -333,10 +331,12 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     done += t_end - t;
     t = t_end;
   }
+  pa_wait_for_previous();
 }
 
 // ---- joining the parts ---------------------------------------------------------------------------------------------------
-// One warp per row: the parts of the prefix and of the sequence's own keys, in the order of their keys.
+// A warp per row, or per four neighbouring rows: the parts of the prefix and of the sequence's own keys, in the order of
+// their keys.  Bound by the chain of lookups (sequence, unit, parts), which four rows share.
 struct PaMergeParams {
   PaCommon c;
   PaPhase own, prefix;       // prefix.prefix_len == 0: none
@@ -364,63 +364,87 @@ __device__ __forceinline__ void pa_load(const float* src, int lane, float* o) {
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int RPW>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant__ PaMergeParams prm) {
+  constexpr int PB = 8 / RPW;             // parts of a row requested before the first is used
   const PaCommon& c = prm.c;
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= (int64_t)c.tokens * c.Hq) return;
-  const int t = (int)(row / c.Hq), hq = (int)(row % c.Hq), h = hq / c.G;
+  const int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * RPW;
+  if (row0 >= (int64_t)c.tokens * c.Hq) return;
+  const int t = (int)(row0 / c.Hq), hq0 = (int)(row0 % c.Hq);
   int b = t;
   if (c.cu) {
     int n = 0;
     for (int i = lane; i < c.B; i += 32) n += c.cu[i + 1] <= t;
     b = __reduce_add_sync(0xffffffffu, n);
   }
+  pa_wait_for_previous();
   if (b >= c.B) return;                   // behind the last sequence: left as it was
-  float m = -INFINITY, l = 0.f, acc[D / 32];
+  float m[RPW], l[RPW], acc[RPW][D / 32];
+  bool skip[RPW];                         // written already
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+  for (int j = 0; j < RPW; ++j) {
+    m[j] = -INFINITY, l[j] = 0.f, skip[j] = false;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[j][i] = 0.f;
+  }
+#pragma unroll 1
   for (int ph = 0; ph < 2; ++ph) {
     const PaPhase& p = ph == 0 ? prm.prefix : prm.own;
     if (ph == 0 && p.prefix_len == 0) continue;
     const int pb = ph == 0 ? 0 : b;
     const PaSeq s = pa_seq(c, p, pb);
-    const long long r = (long long)(t - s.t0) * c.G + hq % c.G;
-    const int rb = (int)(r / p.rows);
-    if (t < s.t0 || t >= s.t0 + s.n || pa_limit(c, p, s, rb) == 0) continue;
-    const int2 who = p.info[pa_unit_id(c, p, pb, s, h, rb)];
-    if (who.x == who.y) {
-      if (p.direct) return;               // already written
-      float o[D / 32];
-      pa_load<D>(p.row_o + row * D, lane, o);
-      pa_take<D>(p.row_ml[row], o, m, l, acc);
-    } else {
-      // eight parts are requested before the first is used
-      const int64_t in_block = r - (long long)rb * p.rows;
-      for (int cta = who.x; cta <= who.y; cta += 8) {
-        float o[8][D / 32];
-        float2 ml[8];
+    if (t < s.t0 || t >= s.t0 + s.n) continue;
+    // where the parts of every row lie: (first CTA, parts); one part in the row arrays, or slots
+    int2 who[RPW];
+    int parts[RPW], in_block[RPW], most = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (cta + k > who.y) break;
-          const int64_t at = (int64_t)(2 * (cta + k) + (cta + k == who.x ? 1 : 0)) * p.rows + in_block;
-          ml[k] = p.slot_ml[at];
-          pa_load<D>(p.slot_o + at * D, lane, o[k]);
+    for (int j = 0; j < RPW; ++j) {
+      const int hq = hq0 + j, h = hq / c.G;
+      const long long r = (long long)(t - s.t0) * c.G + hq % c.G;
+      const int rb = (int)(r / p.rows);
+      in_block[j] = (int)(r - (long long)rb * p.rows);
+      who[j] = pa_limit(c, p, s, rb) == 0 ? make_int2(0, -1) : p.info[pa_unit_id(c, p, pb, s, h, rb)];
+    }
+#pragma unroll
+    for (int j = 0; j < RPW; ++j) {
+      parts[j] = who[j].y - who[j].x + 1;
+      if (parts[j] == 1 && p.direct) parts[j] = 0, skip[j] = true;
+      most = max(most, parts[j]);
+    }
+    for (int k0 = 0; k0 < most; k0 += PB) {
+      float o[RPW][PB][D / 32];
+      float2 ml[RPW][PB];
+#pragma unroll
+      for (int j = 0; j < RPW; ++j)
+#pragma unroll
+        for (int k = 0; k < PB; ++k) {
+          if (k0 + k >= parts[j]) continue;
+          const bool whole = who[j].x == who[j].y;
+          const int cta = who[j].x + k0 + k;
+          const int64_t at = whole ? row0 + j : (int64_t)(2 * cta + (cta == who[j].x ? 1 : 0)) * p.rows + in_block[j];
+          ml[j][k] = (whole ? p.row_ml : p.slot_ml)[at];
+          pa_load<D>((whole ? p.row_o : p.slot_o) + at * D, lane, o[j][k]);
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (cta + k <= who.y) pa_take<D>(ml[k], o[k], m, l, acc);
-      }
+      for (int j = 0; j < RPW; ++j)
+#pragma unroll
+        for (int k = 0; k < PB; ++k)
+          if (k0 + k < parts[j]) pa_take<D>(ml[j][k], o[j][k], m[j], l[j], acc[j]);
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* dst = reinterpret_cast<T*>(c.out) + (int64_t)t * c.o_st + (int64_t)hq * c.o_sh + lane * (D / 32);
-  if (D == 128)
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pa_pack<T>(acc[0] * inv, acc[1] * inv), pa_pack<T>(acc[2] * inv, acc[D / 32 - 1] * inv));
-  else
-    *reinterpret_cast<uint32_t*>(dst) = pa_pack<T>(acc[0] * inv, acc[1] * inv);
-  if (c.lse && lane == 0) c.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+#pragma unroll
+  for (int j = 0; j < RPW; ++j) {
+    if (skip[j]) continue;
+    const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];
+    T* dst = reinterpret_cast<T*>(c.out) + (int64_t)t * c.o_st + (int64_t)(hq0 + j) * c.o_sh + lane * (D / 32);
+    const float* a = acc[j];
+    if (D == 128)
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pa_pack<T>(a[0] * inv, a[1] * inv), pa_pack<T>(a[2] * inv, a[D / 32 - 1] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(dst) = pa_pack<T>(a[0] * inv, a[1] * inv);
+    if (c.lse && lane == 0) c.lse[row0 + j] = l[j] == 0.f ? -INFINITY : (m[j] + log2f(l[j])) * 0.6931471805599453f;
+  }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
@@ -484,24 +508,37 @@ static PaPlan pa_plan(const fa_paged_attn_args_t* a) {
   return pl;
 }
 
+// `after`: may begin while the launch before drains
+template <typename P>
+static int pa_launch(void (*kernel)(P), const P& prm, unsigned grid, int threads, int smem, bool after, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, prm);
+  return e == cudaSuccess ? FA_OK : cuda_fail(e, "fa_paged_attn");
+}
+
 template <typename T, int D, int NT>
-static int pa_stream_launch(const PaStreamParams& prm, cudaStream_t st) {
+static int pa_stream_launch(const PaStreamParams& prm, bool second, cudaStream_t st) {
   constexpr int smem = PaStream<D>::SMEM;
   const int rc = allow_smem<paged_stream_kernel<T, D, NT>>(smem, "cudaFuncSetAttribute(paged_stream)");
   if (rc != FA_OK) return rc;
-  paged_stream_kernel<T, D, NT><<<prm.p.ctas, 256, smem, st>>>(prm);
-  FA_CHECK_LAUNCH("fa_paged_attn");
-  return FA_OK;
+  return pa_launch(paged_stream_kernel<T, D, NT>, prm, prm.p.ctas, 256, smem, second, st);
 }
 
 template <typename T, int D>
-static int pa_tile_launch(const PaTileParams& prm, cudaStream_t st) {
+static int pa_tile_launch(const PaTileParams& prm, bool second, cudaStream_t st) {
   constexpr int smem = PaTile<D>::SMEM;
   const int rc = allow_smem<paged_tile_kernel<T, D>>(smem, "cudaFuncSetAttribute(paged_tile)");
   if (rc != FA_OK) return rc;
-  paged_tile_kernel<T, D><<<prm.p.ctas, PT_THREADS, smem, st>>>(prm);
-  FA_CHECK_LAUNCH("fa_paged_attn(tile)");
-  return FA_OK;
+  return pa_launch(paged_tile_kernel<T, D>, prm, prm.p.ctas, PT_THREADS, smem, second, st);
 }
 
 template <typename T, int D>
@@ -555,15 +592,17 @@ static int pa_run(const fa_paged_attn_args_t* a, cudaStream_t st) {
   for (int i = shared ? 1 : 0; i >= 0; --i) {
     prm.p = tile.p = phase(i);
     (i == 0 ? mg.own : mg.prefix) = prm.p;
-    rc = prm.p.rows == PT_ROWS ? pa_tile_launch<T, D>(tile, st)
-         : prm.p.rows == 8     ? pa_stream_launch<T, D, 1>(prm, st)
-                               : pa_stream_launch<T, D, 2>(prm, st);
+    const bool second = shared && i == 0;
+    rc = prm.p.rows == PT_ROWS ? pa_tile_launch<T, D>(tile, second, st)
+         : prm.p.rows == 8     ? pa_stream_launch<T, D, 1>(prm, second, st)
+                               : pa_stream_launch<T, D, 2>(prm, second, st);
     if (rc != FA_OK) return rc;
   }
   const int64_t rows = (int64_t)a->tokens * a->Hq;
-  paged_merge_kernel<T, D><<<(unsigned)ceil_div64(rows, 8), 256, 0, st>>>(mg);
-  FA_CHECK_LAUNCH("fa_paged_attn(merge)");
-  return FA_OK;
+  // four rows per warp once every SM has work of that kind for all of its warps
+  if (a->Hq % 4 == 0 && rows >= 4 * 32 * (int64_t)sm_count())
+    return pa_launch(paged_merge_kernel<T, D, 4>, mg, (unsigned)ceil_div64(rows, 32), 256, 0, true, st);
+  return pa_launch(paged_merge_kernel<T, D, 1>, mg, (unsigned)ceil_div64(rows, 8), 256, 0, true, st);
 }
 
 }  // namespace fa

@@ -187,6 +187,14 @@ __device__ __forceinline__ int pa_owner(const PaRange& r, long long tile) {
   return (int)(((tile + 1) * r.ctas - 1) / r.total);
 }
 
+// ---- the launches of one call ----------------------------------------------------------------------------------------
+// The kernel over the prefix, the one over the sequences' own keys and the merge are launched so that each may begin
+// while the one before drains (programmatic stream serialization).  The first two share nothing but the output of
+// earlier launches; the second waits for the first before it ends, so that the merge, which waits for the second,
+// finds both results complete.
+__device__ __forceinline__ void pa_let_next_begin() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+__device__ __forceinline__ void pa_wait_for_previous() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+
 // ---- PTX -----------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t pa_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void pa_bar_init(uint32_t bar, int count) {

@@ -199,6 +199,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
   pt_before();
+  pa_let_next_begin();
   PaUnit u;
   int t;
   const PaRange range = pa_locate<PT_THREADS>(c, p, blockIdx.x, sh.loc, u, t);   // two block barriers
@@ -537,6 +538,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     pt_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
   }
+  pa_wait_for_previous();
 }
 
 }  // namespace fa
