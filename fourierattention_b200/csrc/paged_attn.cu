@@ -95,49 +95,53 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
   // ---- this warp's fetches: the same walk as below, ST groups of 16 keys ahead -----------------------------------------
   PaUnit fu = u;
   int ft = t, f_left = (int)(range.end - range.beg);
-  int f_tok = 0, f_page = 0;
-  bool f_have = false;
-  auto f_next = [&]() {
-    f_have = false;
+  struct Fetch {
+    int tok, page, head;                  // tok < 0: nothing left
+  };
+  auto f_next = [&]() -> Fetch {
     while (f_left > 0) {
       if (ft >= fu.tiles) {
         fu.next(c, p);
         ft = 0;
         continue;
       }
-      f_tok = ft * PA_TILE + warp * 16;
+      const int tok = ft * PA_TILE + warp * 16;
       ++ft, --f_left;
-      if (f_tok < fu.limit) {
-        f_have = true;
-        f_page = p.table[(int64_t)fu.b * p.table_sb + f_tok / c.page_size];
-        return;
-      }
+      if (tok < fu.limit)
+        return Fetch{tok, p.table[(int64_t)fu.b * p.table_sb + (unsigned)tok / (unsigned)c.page_size], fu.h};
     }
+    return Fetch{-1, 0, 0};
   };
   uint32_t bad = 0;                       // stages whose page id names no page
-  auto fetch = [&](int stage) {
-    if (!f_have) return;
-    const bool ok = f_page >= 0 && f_page < c.num_pages;
+  auto issue = [&](const Fetch& f, int stage) {
+    if (f.tok < 0) return;
+    const bool ok = f.page >= 0 && f.page < c.num_pages;
     bad = ok ? bad & ~(1u << stage) : bad | (1u << stage);
     if (lane == 0) {
       const uint32_t bar = bar0 + 8 * stage, dst = ring + stage * C::STAGE;
       if (ok) {
-        const int row = f_tok % c.page_size;
+        const int row = (int)((unsigned)f.tok % (unsigned)c.page_size);
         pa_bar_expect(bar, C::STAGE);
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
-          pa_tma(dst + i * C::BOX, &prm.tm_k, 64 * i, row, fu.h, f_page, bar);
-          pa_tma(dst + C::STAGE / 2 + i * C::BOX, &prm.tm_v, 64 * i, row, fu.h, f_page, bar);
+          pa_tma(dst + i * C::BOX, &prm.tm_k, 64 * i, row, f.head, f.page, bar);
+          pa_tma(dst + C::STAGE / 2 + i * C::BOX, &prm.tm_v, 64 * i, row, f.head, f.page, bar);
         }
       } else {
         pa_bar_arrive(bar);
       }
     }
-    f_next();
   };
-  f_next();
-#pragma unroll 1
-  for (int s = 0; s < C::ST; ++s) fetch(s);
+  // the page ids of the first groups are requested together, later ones a group ahead
+  Fetch ahead;
+  {
+    Fetch f[C::ST];
+#pragma unroll
+    for (int s = 0; s < C::ST; ++s) f[s] = f_next();
+    ahead = f_next();
+#pragma unroll
+    for (int s = 0; s < C::ST; ++s) issue(f[s], s);
+  }
 
   const int g = lane >> 2, c2 = 2 * (lane & 3);
   const int ld_row = lane & 15, ld_half = lane >> 4;                       // K: rows as they lie
@@ -154,8 +158,8 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     }
     const int t_end = (int)min((long long)u.tiles, t + (range.end - done));
     // ---- the block's query rows, as the second operand -------------------------------------------------------------
-    const int row0 = u.rb * p.rows;
-    const int n_rows = (int)min((long long)p.rows, (long long)u.s.n * c.G - row0);
+    const int row0 = u.rb << p.rows_log2;
+    const int n_rows = min(1 << p.rows_log2, u.s.n * c.G - row0);
     uint32_t qf[NT][D / 16][2];
     int lim[NT][2];
 #pragma unroll
@@ -261,7 +265,8 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
         }
       }
       __syncwarp();                       // every lane has read the stage
-      fetch(stage);
+      issue(ahead, stage);
+      ahead = f_next();
       if (++stage == C::ST) stage = 0, parity ^= 1;
     }
 
@@ -317,7 +322,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
             c.lse[(int64_t)tok * c.Hq + hq] = lsum == 0.f ? -INFINITY : (mx + log2f(lsum)) * 0.6931471805599453f;
         } else {
           const int64_t at = whole ? (int64_t)tok * c.Hq + hq
-                                   : (int64_t)(2 * blockIdx.x + (first ? 1 : 0)) * p.rows + r;
+                                   : ((int64_t)(2 * blockIdx.x + (first ? 1 : 0)) << p.rows_log2) + r;
           *reinterpret_cast<float4*>((whole ? p.row_o : p.slot_o) + at * D + d4) = acc;
           if (d4 == 0) (whole ? p.row_ml : p.slot_ml)[at] = make_float2(mx, lsum);
         }
@@ -342,17 +347,6 @@ struct PaMergeParams {
   PaPhase own, prefix;       // prefix.prefix_len == 0: none
 };
 
-// One part into the running sums.
-template <int D>
-__device__ __forceinline__ void pa_take(float2 ml, const float* o, float& m, float& l, float* acc) {
-  const float mx = fmaxf(m, ml.x);
-  if (mx == -INFINITY) return;
-  const float f0 = pa_ex2(m - mx), f1 = pa_ex2(ml.x - mx);
-  l = l * f0 + ml.y * f1;
-  m = mx;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = acc[i] * f0 + o[i] * f1;
-}
 template <int D>
 __device__ __forceinline__ void pa_load(const float* src, int lane, float* o) {
   if (D == 128) {
@@ -371,7 +365,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
   const int lane = threadIdx.x & 31;
   const int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * RPW;
   if (row0 >= (int64_t)c.tokens * c.Hq) return;
-  const int t = (int)(row0 / c.Hq), hq0 = (int)(row0 % c.Hq);
+  const int t = (int)((unsigned)row0 / (unsigned)c.Hq), hq0 = (int)row0 - t * c.Hq;
   int b = t;
   if (c.cu) {
     int n = 0;
@@ -380,57 +374,86 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
   }
   pa_wait_for_previous();
   if (b >= c.B) return;                   // behind the last sequence: left as it was
+  // Where the parts of every row lie, in both phases at once: (first CTA, last); one part in the row arrays, or slots.
+  int2 who[2][RPW];
+  int in_block[2][RPW];
+  PaSeq s[2];
+#pragma unroll
+  for (int ph = 0; ph < 2; ++ph) s[ph] = pa_seq(c, ph == 0 ? prm.prefix : prm.own, ph == 0 ? 0 : b);
+#pragma unroll
+  for (int ph = 0; ph < 2; ++ph) {
+    const PaPhase& p = ph == 0 ? prm.prefix : prm.own;
+    const bool on = (ph == 1 || p.prefix_len > 0) && t >= s[ph].t0 && t < s[ph].t0 + s[ph].n;
+#pragma unroll
+    for (int j = 0; j < RPW; ++j) {
+      const int hq = hq0 + j, h = hq / c.G;
+      const int r = (t - s[ph].t0) * c.G + hq - h * c.G, rb = r >> p.rows_log2;
+      in_block[ph][j] = r - (rb << p.rows_log2);
+      who[ph][j] = make_int2(0, -1);
+      if (on && pa_unit_tiles(p, pa_limit(c, p, s[ph], rb)) > 0)
+        who[ph][j] = p.info[pa_unit_id(c, p, ph == 0 ? 0 : b, s[ph], h, rb)];
+    }
+  }
   float m[RPW], l[RPW], acc[RPW][D / 32];
   bool skip[RPW];                         // written already
 #pragma unroll
   for (int j = 0; j < RPW; ++j) {
-    m[j] = -INFINITY, l[j] = 0.f, skip[j] = false;
+    m[j] = -INFINITY, l[j] = 0.f;
+    skip[j] = prm.own.direct && who[1][j].x == who[1][j].y;
+    if (skip[j]) who[1][j].y = who[1][j].x - 1;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) acc[j][i] = 0.f;
   }
-#pragma unroll 1
+#pragma unroll
   for (int ph = 0; ph < 2; ++ph) {
     const PaPhase& p = ph == 0 ? prm.prefix : prm.own;
-    if (ph == 0 && p.prefix_len == 0) continue;
-    const int pb = ph == 0 ? 0 : b;
-    const PaSeq s = pa_seq(c, p, pb);
-    if (t < s.t0 || t >= s.t0 + s.n) continue;
-    // where the parts of every row lie: (first CTA, parts); one part in the row arrays, or slots
-    int2 who[RPW];
-    int parts[RPW], in_block[RPW], most = 0;
+    int most = 0;
 #pragma unroll
-    for (int j = 0; j < RPW; ++j) {
-      const int hq = hq0 + j, h = hq / c.G;
-      const long long r = (long long)(t - s.t0) * c.G + hq % c.G;
-      const int rb = (int)(r / p.rows);
-      in_block[j] = (int)(r - (long long)rb * p.rows);
-      who[j] = pa_limit(c, p, s, rb) == 0 ? make_int2(0, -1) : p.info[pa_unit_id(c, p, pb, s, h, rb)];
-    }
+    for (int j = 0; j < RPW; ++j) most = max(most, who[ph][j].y - who[ph][j].x + 1);
+    for (int base = 0; base < most; base += 32) {
+      // maximum and denominator of up to 32 parts, a part per lane; then the parts' weights
+      auto place = [&](int j, int k) -> int64_t {
+        const int2 w = who[ph][j];
+        const int cta = w.x + k;
+        return w.x == w.y ? row0 + j : ((int64_t)(2 * cta + (cta == w.x ? 1 : 0)) << p.rows_log2) + in_block[ph][j];
+      };
+      float2 ml[RPW];
 #pragma unroll
-    for (int j = 0; j < RPW; ++j) {
-      parts[j] = who[j].y - who[j].x + 1;
-      if (parts[j] == 1 && p.direct) parts[j] = 0, skip[j] = true;
-      most = max(most, parts[j]);
-    }
-    for (int k0 = 0; k0 < most; k0 += PB) {
-      float o[RPW][PB][D / 32];
-      float2 ml[RPW][PB];
+      for (int j = 0; j < RPW; ++j) {
+        ml[j] = make_float2(-INFINITY, 0.f);
+        const int2 w = who[ph][j];
+        if (w.x + base + lane <= w.y) ml[j] = (w.x == w.y ? p.row_ml : p.slot_ml)[place(j, base + lane)];
+      }
+      float weight[RPW];
 #pragma unroll
-      for (int j = 0; j < RPW; ++j)
+      for (int j = 0; j < RPW; ++j) {
+        const float mx = fmaxf(m[j], warp_max(ml[j].x));
+        const float f = m[j] == -INFINITY ? 0.f : pa_ex2(m[j] - mx);
+        weight[j] = ml[j].x == -INFINITY ? 0.f : pa_ex2(ml[j].x - mx);
+        if (ml[j].x != ml[j].x) weight[j] = ml[j].x;                    // a part that gave up poisons its rows
+        m[j] = mx;
+        l[j] = l[j] * f + warp_sum(weight[j] * ml[j].y);
 #pragma unroll
-        for (int k = 0; k < PB; ++k) {
-          if (k0 + k >= parts[j]) continue;
-          const bool whole = who[j].x == who[j].y;
-          const int cta = who[j].x + k0 + k;
-          const int64_t at = whole ? row0 + j : (int64_t)(2 * cta + (cta == who[j].x ? 1 : 0)) * p.rows + in_block[j];
-          ml[j][k] = (whole ? p.row_ml : p.slot_ml)[at];
-          pa_load<D>((whole ? p.row_o : p.slot_o) + at * D, lane, o[j][k]);
-        }
+        for (int i = 0; i < D / 32; ++i) acc[j][i] *= f;
+      }
+      for (int k0 = base; k0 < min(most, base + 32); k0 += PB) {
+        float o[RPW][PB][D / 32];
 #pragma unroll
-      for (int j = 0; j < RPW; ++j)
+        for (int j = 0; j < RPW; ++j)
 #pragma unroll
-        for (int k = 0; k < PB; ++k)
-          if (k0 + k < parts[j]) pa_take<D>(ml[j][k], o[j][k], m[j], l[j], acc[j]);
+          for (int k = 0; k < PB; ++k)
+            if (who[ph][j].x + k0 + k <= who[ph][j].y)
+              pa_load<D>((who[ph][j].x == who[ph][j].y ? p.row_o : p.slot_o) + place(j, k0 + k) * D, lane, o[j][k]);
+#pragma unroll
+        for (int j = 0; j < RPW; ++j)
+#pragma unroll
+          for (int k = 0; k < PB; ++k) {
+            const float w = __shfl_sync(0xffffffffu, weight[j], (k0 + k - base) & 31);
+            if (who[ph][j].x + k0 + k <= who[ph][j].y)
+#pragma unroll
+              for (int i = 0; i < D / 32; ++i) acc[j][i] = fmaf(o[j][k][i], w, acc[j][i]);
+          }
+      }
     }
   }
 #pragma unroll
@@ -465,7 +488,7 @@ static int pa_check(const fa_paged_attn_args_t* a) {
              "%s: the page size must be a multiple of 16 (got %d)", w, a->page_size);
   FA_REQUIRE((int64_t)a->max_pages * a->page_size < (1ll << 31) - PA_TILE, FA_ERR_CAPACITY,
              "%s: a sequence of up to %lld keys", w, (long long)a->max_pages * a->page_size);
-  FA_REQUIRE((int64_t)a->tokens * (a->Hq / a->Hkv) < (1ll << 31) - 4096, FA_ERR_CAPACITY, "%s: too many query rows", w);
+  FA_REQUIRE((int64_t)a->tokens * a->Hq < (1ll << 31) - 4096, FA_ERR_CAPACITY, "%s: too many query rows", w);
   FA_REQUIRE(a->cu_seqlens || a->tokens == a->B, FA_ERR_SHAPE,
              "%s: without cu_seqlens there is one token per sequence (%d tokens, %d sequences)", w, a->tokens, a->B);
   FA_REQUIRE((int64_t)a->prefix_len < (1ll << 31) - PA_TILE && (a->prefix_len == 0 || (int64_t)a->n_prefix_pages * a->page_size >= a->prefix_len),
@@ -475,6 +498,7 @@ static int pa_check(const fa_paged_attn_args_t* a) {
 
 struct PaPlan {
   int rows_own, rows_pre, ctas;
+  bool lead;                  // the prefix in front of every sequence's own keys, not as a phase of its own
   size_t bytes, slot_o[2], slot_ml[2], row_o[2], row_ml[2], info[2];
 };
 
@@ -483,7 +507,7 @@ static PaPlan pa_plan(const fa_paged_attn_args_t* a) {
   const int64_t G = a->Hq / a->Hkv;
   pl.ctas = sm_count();
   // eight rows fill the streaming kernel's instruction; sixteen take a second one per key; more go to the tile kernel
-  const int64_t own = a->cu_seqlens ? (int64_t)a->tokens * G / a->B : G, pre = (int64_t)a->tokens * G;
+  const int64_t own = a->cu_seqlens && a->B > 0 ? (int64_t)a->tokens * G / a->B : G, pre = (int64_t)a->tokens * G;
   pl.rows_own = a->cu_seqlens && own > 16 ? PT_ROWS : own <= 8 ? 8 : 16;
   pl.rows_pre = pre > 16 ? PT_ROWS : pre <= 8 ? 8 : 16;
   size_t at = 0;
@@ -492,7 +516,11 @@ static PaPlan pa_plan(const fa_paged_attn_args_t* a) {
     at += (n + 255) / 256 * 256;
     return r;
   };
-  const bool shared = a->prefix_len > 0;
+  // Blocks that a sequence's own rows fill read the prefix no more often by themselves than packed with others', and the
+  // prefix in front of their own keys saves a launch, the partial results and the merge (8 x up to 250 tokens of 4 heads
+  // per group over 16384 keys: 503 us as two phases); emptier blocks are better packed across the batch.
+  pl.lead = a->prefix_len > 0 && pl.rows_own == PT_ROWS && own >= 3 * PT_ROWS / 4;
+  const bool shared = a->prefix_len > 0 && !pl.lead;
   for (int i = 0; i < (shared ? 2 : 1); ++i) {
     const int64_t rows = i == 0 ? pl.rows_own : pl.rows_pre;
     pl.slot_o[i] = take((size_t)2 * pl.ctas * rows * a->D * 4);
@@ -555,7 +583,7 @@ static int pa_run(const fa_paged_attn_args_t* a, cudaStream_t st) {
   c.page_size = a->page_size, c.num_pages = a->num_pages;
   const float scale = a->sm_scale > 0.f ? a->sm_scale : 1.f / sqrtf((float)D);
   c.scale_log2 = scale * 1.4426950408889634f;
-  const bool shared = a->prefix_len > 0;
+  const bool shared = a->prefix_len > 0 && !pl.lead;
   PaTileParams tile;
   tile.box_rows = 16;
   while (tile.box_rows < PA_TILE && a->page_size % (2 * tile.box_rows) == 0) tile.box_rows *= 2;
@@ -578,7 +606,10 @@ static int pa_run(const fa_paged_attn_args_t* a, cudaStream_t st) {
     p.table_sb = i == 0 ? a->table_sb : 0;
     p.max_pages = i == 0 ? a->max_pages : a->n_prefix_pages;
     p.prefix_len = i == 0 ? 0 : a->prefix_len;
-    p.rows = i == 0 ? pl.rows_own : pl.rows_pre;
+    p.lead_table = a->prefix_pages;
+    p.lead_len = i == 0 && pl.lead ? a->prefix_len : 0;
+    const int rows = i == 0 ? pl.rows_own : pl.rows_pre;
+    p.rows_log2 = rows == PT_ROWS ? 8 : rows == 16 ? 4 : 3;
     p.ctas = pl.ctas;
     p.direct = !shared;
     p.slot_o = reinterpret_cast<float*>(s + pl.slot_o[i]);
@@ -588,14 +619,14 @@ static int pa_run(const fa_paged_attn_args_t* a, cudaStream_t st) {
     p.info = reinterpret_cast<int2*>(s + pl.info[i]);
     return p;
   };
-  mg.prefix.prefix_len = 0;
+  mg.prefix = PaPhase{};
   for (int i = shared ? 1 : 0; i >= 0; --i) {
     prm.p = tile.p = phase(i);
     (i == 0 ? mg.own : mg.prefix) = prm.p;
     const bool second = shared && i == 0;
-    rc = prm.p.rows == PT_ROWS ? pa_tile_launch<T, D>(tile, second, st)
-         : prm.p.rows == 8     ? pa_stream_launch<T, D, 1>(prm, second, st)
-                               : pa_stream_launch<T, D, 2>(prm, second, st);
+    rc = prm.p.rows_log2 == 8   ? pa_tile_launch<T, D>(tile, second, st)
+         : prm.p.rows_log2 == 3 ? pa_stream_launch<T, D, 1>(prm, second, st)
+                                : pa_stream_launch<T, D, 2>(prm, second, st);
     if (rc != FA_OK) return rc;
   }
   const int64_t rows = (int64_t)a->tokens * a->Hq;

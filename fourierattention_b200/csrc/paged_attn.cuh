@@ -19,7 +19,9 @@ struct PaPhase {
   int64_t table_sb;
   int max_pages;
   int prefix_len;            // > 0: the shared prefix, every row sees all of it; 0: each sequence's own pages, causal
-  int rows;                  // rows of a block
+  const int32_t* lead_table; // own pages only: the pages of `lead_len` keys that come before them (tile kernel)
+  int lead_len;
+  int rows_log2;             // rows of a block
   int ctas;
   int direct;                // finished units go straight to `out`
   float* slot_o;             // (2 ctas, rows, D)
@@ -62,27 +64,29 @@ __device__ __forceinline__ PaSeq pa_seq(const PaCommon& c, const PaPhase& p, int
 }
 __device__ __forceinline__ int pa_seqs(const PaCommon& c, const PaPhase& p) { return p.prefix_len > 0 ? 1 : c.B; }
 __device__ __forceinline__ int pa_blocks(const PaCommon& c, const PaPhase& p, const PaSeq& s) {
-  return (int)(((long long)s.n * c.G + p.rows - 1) / p.rows);
+  return (s.n * c.G + (1 << p.rows_log2) - 1) >> p.rows_log2;      // (tokens x G and a block more fit into 31 bits)
 }
 // keys seen by the last row of a block (a later token sees more)
 __device__ __forceinline__ int pa_limit(const PaCommon& c, const PaPhase& p, const PaSeq& s, int rb) {
   if (p.prefix_len > 0) return s.L;
-  const long long last = min((long long)s.n * c.G, (long long)(rb + 1) * p.rows) - 1;
-  return (int)max(0LL, min((long long)s.L, s.L - s.n + last / c.G + 1));
+  const int last = min(s.n * c.G, (rb + 1) << p.rows_log2) - 1;
+  return max(0, min(s.L, s.L - s.n + (int)((unsigned)last / (unsigned)c.G) + 1));
 }
 __device__ __forceinline__ int pa_tiles(int limit) { return (limit + PA_TILE - 1) / PA_TILE; }
+// tiles of a unit whose rows see `limit` keys; those of the lead come first, in tiles of their own
+__device__ __forceinline__ int pa_unit_tiles(const PaPhase& p, int limit) { return pa_tiles(p.lead_len) + pa_tiles(limit); }
 __device__ __forceinline__ long long pa_head_tiles(const PaCommon& c, const PaPhase& p, const PaSeq& s) {
   const int nb = pa_blocks(c, p, s);
   if (nb == 0) return 0;
   if (p.prefix_len > 0) return (long long)nb * pa_tiles(s.L);
   long long sum = 0;
-  for (int rb = 0; rb < nb; ++rb) sum += pa_tiles(pa_limit(c, p, s, rb));
+  for (int rb = 0; rb < nb; ++rb) sum += pa_unit_tiles(p, pa_limit(c, p, s, rb));
   return sum;
 }
 // number of a unit for `info`: distinct, and below pa_info_count()
 __device__ __forceinline__ long long pa_unit_id(const PaCommon& c, const PaPhase& p, int b, const PaSeq& s, int h, int rb) {
-  const long long f0 = (long long)s.t0 * c.G / p.rows + b, f1 = (long long)(s.t0 + s.n) * c.G / p.rows + b + 1;
-  return f0 * c.Hkv + h * (f1 - f0) + rb;
+  const int f0 = ((s.t0 * c.G) >> p.rows_log2) + b, f1 = (((s.t0 + s.n) * c.G) >> p.rows_log2) + b + 1;
+  return (long long)f0 * c.Hkv + h * (f1 - f0) + rb;
 }
 inline int64_t pa_info_count(int64_t tokens, int64_t B, int64_t G, int64_t Hkv, int64_t rows) {
   return (tokens * G / rows + B + 1) * Hkv;
@@ -94,7 +98,7 @@ struct PaUnit {
   PaSeq s;
   __device__ __forceinline__ void set(const PaCommon& c, const PaPhase& p) {
     limit = pa_limit(c, p, s, rb);
-    tiles = pa_tiles(limit);
+    tiles = pa_unit_tiles(p, limit);
   }
   __device__ __forceinline__ void next(const PaCommon& c, const PaPhase& p) {
     if (++rb >= nb) {
@@ -127,6 +131,11 @@ struct PaLocate {              // shared memory of pa_locate()
   int b;
 };
 
+// a / b, b > 0: by the short division where both fit 32 bits
+__device__ __forceinline__ long long pa_div(long long a, long long b) {
+  return ((unsigned long long)a >> 32) == 0 && ((unsigned long long)b >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+
 // Finds this CTA's range of tiles and the unit it begins in (tile `t` of it).  One block-wide scan over the sequences.
 template <int THREADS>
 __device__ __forceinline__ PaRange pa_locate(const PaCommon& c, const PaPhase& p, int cta, PaLocate& sh, PaUnit& u, int& t) {
@@ -154,7 +163,7 @@ __device__ __forceinline__ PaRange pa_locate(const PaCommon& c, const PaPhase& p
   pre += inc - mine;
   r.ctas = (int)min((long long)p.ctas, r.total);
   r.beg = r.end = 0;
-  if (cta < r.ctas) r.beg = r.total * cta / r.ctas, r.end = r.total * (cta + 1) / r.ctas;
+  if (cta < r.ctas) r.beg = pa_div(r.total * cta, r.ctas), r.end = pa_div(r.total * (cta + 1), r.ctas);
   if (r.beg < r.end && pre <= r.beg && r.beg < pre + mine) {
     long long off = r.beg - pre;
     int b = b0;
@@ -171,7 +180,7 @@ __device__ __forceinline__ PaRange pa_locate(const PaCommon& c, const PaPhase& p
   u.s = pa_seq(c, p, u.b);
   u.nb = pa_blocks(c, p, u.s);
   const long long per = pa_head_tiles(c, p, u.s);
-  u.h = (int)(sh.off / per);
+  u.h = (int)pa_div(sh.off, per);
   long long off = sh.off - u.h * per;
   u.rb = 0;
   u.set(c, p);
@@ -184,7 +193,7 @@ __device__ __forceinline__ PaRange pa_locate(const PaCommon& c, const PaPhase& p
   return r;
 }
 __device__ __forceinline__ int pa_owner(const PaRange& r, long long tile) {
-  return (int)(((tile + 1) * r.ctas - 1) / r.total);
+  return (int)pa_div((tile + 1) * r.ctas - 1, r.total);
 }
 
 // ---- the launches of one call ----------------------------------------------------------------------------------------

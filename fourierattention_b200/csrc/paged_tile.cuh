@@ -13,7 +13,8 @@
 //                    `lane == 0`, with descriptors made per MMA, it took 100 to 160 and bound the kernel (an MMA of
 //                    128 x 128 x 16 runs 64)
 //   warp 17          fetches K and V tiles by TMA, a page's rows at a time, into a ring of 32 KB slots
-//   warps 18, 19     complete the warpgroup that gives its registers away
+//   warp 18          walks ahead of the softmax warps and writes down what they work on next
+//   warp 19          completes the warpgroup that gives its registers away
 // Tensor memory (512 columns): S0, S1 (128 each; P overwrites the first half of its S), O0, O1.  MMAs execute in the order
 // of their issue, so S of the next tile may be issued behind the product that still reads P.  The running maximum moves
 // only when a row passes it by 2^8; then the row's thread rescales its accumulator in tensor memory, which nothing else
@@ -27,19 +28,14 @@ namespace fa {
 
 constexpr int PT_THREADS = 640;                           // 96 registers each at launch, moved to where they are needed:
 constexpr int PT_SOFTMAX_REGS = 104, PT_OTHER_REGS = 64;   // 512 x 104 + 128 x 64 = 640 x 96
-constexpr int PT_ROWS = 256;
+constexpr int PT_ROWS = 256;                              // rows_log2 = 8
 
-// what a softmax warpgroup works on next, and where its walk stands: kept in shared memory by the warpgroup's first
-// thread, so that the walk takes no registers from the 128 scores of every thread
+// a stretch of one unit's tiles, as the softmax warps need it; written ahead by a warp of its own, so that the walk and
+// its loads are off their path and take none of their registers
 struct PtSegment {
   int more, row0, t0, n, L, h, t, t_end, first, last;   // more = 0: done
 };
-struct PtWalk {
-  PaUnit u;
-  PaRange r;
-  long long done;
-  int t;
-};
+constexpr int PT_SEGS = 4;
 
 template <int D>
 struct PaTile {
@@ -51,8 +47,8 @@ struct PaTile {
     uint64_t full[ST], empty[ST], q_full[2], s_full[2], p_full[2], o_full[2], tail;
     uint32_t bad[16];          // keys of a tile that no page holds, by groups of 16; the fetches are < 16 tiles ahead
     PaLocate loc;
-    PtWalk walk[2];
-    PtSegment seg[2];
+    PtSegment seg[PT_SEGS];
+    uint64_t seg_full[PT_SEGS], seg_empty[PT_SEGS];
     float half[2][2][128];     // what the two halves of a row tell each other
     uint32_t tmem;
     int dead;
@@ -192,6 +188,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
       pa_bar_init(pa_smem(&sh.o_full[w]), 1);
     }
     pa_bar_init(pa_smem(&sh.tail), 1);
+    for (int s = 0; s < PT_SEGS; ++s) {
+      pa_bar_init(pa_smem(&sh.seg_full[s]), 1);
+      pa_bar_init(pa_smem(&sh.seg_empty[s]), 16);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 16) {
@@ -215,32 +215,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     const uint32_t ts = tmem + w * 128 + lanes, to = tmem + 256 + w * 128 + lanes;
     const uint32_t s_full = pa_smem(&sh.s_full[w]), p_full = pa_smem(&sh.p_full[w]);
     const float scale = c.scale_log2;
-    PtWalk& walk = sh.walk[w];
-    PtSegment& seg = sh.seg[w];
-    if (i == 0 && half == 0) walk.u = u, walk.r = range, walk.done = range.beg, walk.t = t;
     uint32_t s_par = 0, o_par = 0;
     int tile_no = 0;                                      // tiles since the start
-    for (;;) {
-      if (i == 0 && half == 0) {
-        seg.more = walk.done < walk.r.end;
-        if (seg.more) {
-          while (walk.t >= walk.u.tiles) walk.u.next(c, p), walk.t = 0;
-          const PaUnit& x = walk.u;
-          seg.t = walk.t;
-          seg.t_end = (int)min((long long)x.tiles, walk.t + (walk.r.end - walk.done));
-          seg.row0 = x.rb * PT_ROWS + w * 128;
-          seg.t0 = x.s.t0, seg.n = x.s.n, seg.L = x.s.L, seg.h = x.h;
-          seg.first = seg.t == 0, seg.last = seg.t_end == x.tiles;
-          if (seg.last && w == 0)
-            p.info[pa_unit_id(c, p, x.b, x.s, x.h, x.rb)] = make_int2(pa_owner(walk.r, walk.done - walk.t), blockIdx.x);
-          walk.done += seg.t_end - seg.t;
-          walk.t = seg.t_end;
-        }
-      }
-      pt_sync(1 + w);
-      if (!seg.more) break;
-      const int t_beg = seg.t, t_end = seg.t_end, row0 = seg.row0;
-      const int n_rows = (int)max(0LL, min(128LL, (long long)seg.n * c.G - row0));
+    for (int seg_no = 0;; ++seg_no) {
+      const PtSegment& seg = sh.seg[seg_no % PT_SEGS];
+      pa_bar_wait(pa_smem(&sh.seg_full[seg_no % PT_SEGS]), (seg_no / PT_SEGS) & 1, dead);
+      // (by vote: after a wait that gave up the threads may not see alike, and barriers follow)
+      if (pt_sync_any(1 + w, *dead || !seg.more)) break;
+      const int t_beg = seg.t, t_end = seg.t_end, row0 = seg.row0 + w * 128;
+      const int n_rows = max(0, min(128, seg.n * c.G - row0));
       if (n_rows == 0) {
         tile_no += t_end - t_beg;
       } else {
@@ -248,16 +231,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         const uint32_t qb = q_smem + w * C::SLOT;
         {
           const T* q = reinterpret_cast<const T*>(c.q) + (int64_t)seg.t0 * c.q_st + (int64_t)seg.h * c.G * c.q_sh;
-#pragma unroll 4
-          for (int e = half * 128 + i; e < 128 * (D / 8); e += 256) {
-            const int r = e / (D / 8), ch = e % (D / 8);
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < n_rows) {
-              const int tok = (row0 + r) / c.G, hg = (row0 + r) - tok * c.G;
-              v = *reinterpret_cast<const uint4*>(q + (int64_t)tok * c.q_st + (int64_t)hg * c.q_sh + ch * 8);
-            }
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(qb + (ch >> 3) * C::HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
-                         "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+          // a thread takes a half of row i, all of it requested at once
+          constexpr int NQ = D / 16;
+          const int tok = (int)((unsigned)(row0 + i) / (unsigned)c.G), hg = row0 + i - tok * c.G;
+          const uint4* src = reinterpret_cast<const uint4*>(q + (int64_t)tok * c.q_st + (int64_t)hg * c.q_sh) + half * NQ;
+          uint4 v[NQ];
+#pragma unroll
+          for (int k = 0; k < NQ; ++k) v[k] = i < n_rows ? src[k] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int k = 0; k < NQ; ++k) {
+            const int ch = half * NQ + k;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(qb + (ch >> 3) * C::HALF + i * 128 + (((ch & 7) ^ (i & 7)) << 4)),
+                         "r"(v[k].x), "r"(v[k].y), "r"(v[k].z), "r"(v[k].w) : "memory");
           }
         }
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // generic writes -> MMA reads
@@ -266,10 +251,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         if (lane == 0) pa_bar_arrive(pa_smem(&sh.q_full[w]));
 
         const int lim = p.prefix_len > 0 ? seg.L : min(seg.L, seg.L - seg.n + (row0 + min(i, n_rows - 1)) / c.G + 1);
-        int nv = lim - t_beg * PA_TILE - 64 * half;       // keys of this half of the tile that the row sees
+        // keys of this half of the tile that the row sees, counted from the lead's or the sequence's first key
+        const int lead = pa_tiles(p.lead_len);
+        int tt = t_beg;
         float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-        for (int left = t_end - t_beg; left > 0; --left, nv -= PA_TILE) {
+        for (; tt < t_end; ++tt) {
+          const int nv = (tt < lead ? p.lead_len - tt * PA_TILE : lim - (tt - lead) * PA_TILE) - 64 * half;
           pa_bar_wait(s_full, s_par, dead);
           s_par ^= 1;
           pt_after();
@@ -298,7 +286,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             const float f = m == -INFINITY ? 0.f : pa_ex2(m - nm);
             m = nm;
             l *= f;
-            if (left < t_end - t_beg) {
+            if (tt > t_beg) {
 #pragma unroll 1
               for (int j = half * (D / 2); j < (half + 1) * (D / 2); j += 16) {
                 uint32_t o[16];
@@ -360,9 +348,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
 #pragma unroll
             for (int k = 0; k < 4; ++k) dst[k] = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
           } else {
-            uint4* dst = reinterpret_cast<uint4*>((whole ? p.row_o : p.slot_o) + at * D + j);
+            float* dst = (whole ? p.row_o : p.slot_o) + at * D + j;      // a whole 32-byte sector per lane and store
 #pragma unroll
-            for (int k = 0; k < 8; ++k) dst[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            for (int k = 0; k < 32; k += 8)
+              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst + k), PT_W8(o, k) : "memory");
           }
         }
         if (i < n_rows && half == 0) {
@@ -374,7 +363,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         }
         pt_before();
       }
-      pt_sync(1 + w);   // everyone has read the segment
+      __syncwarp();
+      if (lane == 0) pa_bar_arrive(pa_smem(&sh.seg_empty[seg_no % PT_SEGS]));   // read
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PT_OTHER_REGS));
@@ -387,6 +377,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     const uint64_t q_desc = pt_desc(q_smem, 16, 1024), k_desc = pt_desc(ring, 16, 1024), v_desc = pt_desc(ring, C::HALF, 1024);
     int slot = 0;
     uint32_t par = 0, q_par = 0, p_par = 0;               // q_par, p_par: a bit per query tile
+    const int lead = pa_tiles(p.lead_len);
     auto advance = [&]() {
       if (++slot == C::ST) slot = 0, par ^= 1;
     };
@@ -410,7 +401,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         continue;
       }
       const int t_end = (int)min((long long)u.tiles, t + (range.end - done));
-      const int nw = (long long)u.s.n * c.G - (long long)u.rb * PT_ROWS > 128 ? 2 : 1;
+      const int nw = u.s.n * c.G - u.rb * PT_ROWS > 128 ? 2 : 1;
       // K of the first tile
       pa_bar_wait(pa_smem(&sh.full[slot]), par, dead);
       for (int w = 0; w < nw; ++w) {
@@ -424,7 +415,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
       advance();
       for (int tt = t; tt < t_end; ++tt) {
         const bool more = tt + 1 < t_end;
-        const int steps = (min(PA_TILE, u.limit - tt * PA_TILE) + 15) / 16;
+        const int steps = (min(PA_TILE, tt < lead ? p.lead_len - tt * PA_TILE : u.limit - (tt - lead) * PA_TILE) + 15) / 16;
         const int v_slot = slot;
         pa_bar_wait(pa_smem(&sh.full[slot]), par, dead);
         advance();
@@ -467,12 +458,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     // ---- the fetches --------------------------------------------------------------------------------------------------
     int slot = 0, tile_no = 0;
     uint32_t par = 1, t_par = 0;                          // the first pass over the ring finds it empty
-    const int box_keys = prm.box_rows;
+    const int box_keys = prm.box_rows, lead = pa_tiles(p.lead_len);
     const uint32_t box_bytes = box_keys * 128;
     // lane i holds the page id of box i of the tile to come, requested while the tile before is fetched
     auto page_id = [&]() -> int {
-      const int key = t * PA_TILE + lane * box_keys;
-      return lane * box_keys < PA_TILE && key < u.limit ? p.table[(int64_t)u.b * p.table_sb + key / c.page_size] : 0;
+      const int key = (t < lead ? t : t - lead) * PA_TILE + lane * box_keys;
+      if (lane * box_keys >= PA_TILE || key >= (t < lead ? p.lead_len : u.limit)) return 0;
+      return (t < lead ? p.lead_table : p.table + (int64_t)u.b * p.table_sb)[key / c.page_size];
     };
     auto to_tile = [&]() {
       while (done < range.end && t >= u.tiles) u.next(c, p), t = 0;
@@ -480,9 +472,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     to_tile();
     int next_id = done < range.end ? page_id() : 0;
     while (done < range.end) {
-      const int key0 = t * PA_TILE, nv = min(PA_TILE, u.limit - key0);
+      const int key0 = (t < lead ? t : t - lead) * PA_TILE, nv = min(PA_TILE, (t < lead ? p.lead_len : u.limit) - key0);
       const int need = (nv + box_keys - 1) / box_keys;                // boxes with keys
-      const int row = (key0 + lane * box_keys) % c.page_size, head = u.h, L = u.s.L;
+      const int row = (key0 + lane * box_keys) % c.page_size, head = u.h, L = t < lead ? p.lead_len : u.s.L;
       int page = next_id;
       const bool ok = lane >= need || (page >= 0 && page < c.num_pages);
       if (!ok) page = c.num_pages;                        // out of the map's range: zeros arrive
@@ -525,6 +517,29 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         if (++slot == C::ST) slot = 0, par ^= 1;
       }
       ++tile_no;
+    }
+  }
+  if (warp == 18 && lane == 0) {
+    // ---- what the softmax warps work on --------------------------------------------------------------------------------
+    for (int seg_no = 0;; ++seg_no) {
+      const int x = seg_no % PT_SEGS;
+      if (seg_no >= PT_SEGS) pa_bar_wait(pa_smem(&sh.seg_empty[x]), (seg_no / PT_SEGS - 1) & 1, dead);
+      PtSegment seg;
+      seg.more = done < range.end && !*dead;
+      if (seg.more) {
+        while (t >= u.tiles) u.next(c, p), t = 0;
+        seg.t = t;
+        seg.t_end = (int)min((long long)u.tiles, t + (range.end - done));
+        seg.row0 = u.rb * PT_ROWS;
+        seg.t0 = u.s.t0, seg.n = u.s.n, seg.L = u.s.L, seg.h = u.h;
+        seg.first = seg.t == 0, seg.last = seg.t_end == u.tiles;
+      }
+      sh.seg[x] = seg;
+      pa_bar_arrive(pa_smem(&sh.seg_full[x]));
+      if (!seg.more) break;
+      if (seg.last) p.info[pa_unit_id(c, p, u.b, u.s, u.h, u.rb)] = make_int2(pa_owner(range, done - t), blockIdx.x);
+      done += seg.t_end - seg.t;
+      t = seg.t_end;
     }
   }
   if (*dead) {

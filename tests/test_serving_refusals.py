@@ -171,6 +171,8 @@ def test_library_refuses(ops):
         assert call(lib.fa_paged_attn, attn(**kw)) == rc, kw
     assert lib.fa_paged_attn_scratch_bytes(bytes(attn())) > 0
     assert lib.fa_paged_attn_scratch_bytes(bytes(attn(D=96))) == 0
+    for kw in (dict(tokens=0, B=0), dict(tokens=0, B=0, cu_seqlens=4096), dict(tokens=5, B=0, cu_seqlens=4096)):
+        lib.fa_paged_attn_scratch_bytes(bytes(attn(**kw)))          # sizes of nothing: no fault
     one = lambda **kw: lib.fa_sample(*{**dict(x=4096, dt=1, B=2, V=10, sb=10, u=4096, t=None, t0=1.0, k=None, k0=0, p=None, p0=1.0, m=None,
                                               m0=0.0, tok=4096, lp=None, st=None), **kw}.values())
     assert one(dt=3) == -3 and one(V=0) == -2 and one(B=-1) == -2 and one(V=393217) == -5 and one(x=None) == -1
