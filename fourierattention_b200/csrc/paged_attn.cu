@@ -336,6 +336,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     done += t_end - t;
     t = t_end;
   }
+  pa_leave(&sh.dead);
   pa_wait_for_previous();
 }
 

@@ -234,6 +234,12 @@ __device__ __forceinline__ void pa_bar_wait(uint32_t bar, uint32_t parity, volat
     }
   }
 }
+// After a wait that gave up: time for what is still in flight, before shared memory is given back.
+__device__ __forceinline__ void pa_leave(volatile int* dead) {
+  if (!*dead) return;
+  const long long t0 = clock64();
+  while (clock64() - t0 < 20000000LL) __nanosleep(1000);
+}
 __device__ __forceinline__ void pa_tma(uint32_t dst, const CUtensorMap* map, int x, int row, int head, int page,
                                        uint32_t bar) {
   asm volatile(

@@ -542,11 +542,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
       t = seg.t_end;
     }
   }
-  if (*dead) {
-    // a wait gave up: leave time for what is still in flight
-    const long long t0 = clock64();
-    while (clock64() - t0 < 20000000LL) __nanosleep(1000);
-  }
+  pa_leave(dead);
   pt_before();
   __syncthreads();
   if (warp == 16) {

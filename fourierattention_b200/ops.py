@@ -664,6 +664,10 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens=None, p
         raise ValueError("k_pages: expected (num_pages, kv_heads, page_size, head_dim)")
     pages, kp, vp = _pages(k_pages, v_pages, dtype, k_pages.shape[1], D)
     B, most = _sequences(page_table, kv_lens, cu_seqlens, tokens)
+    if sm_scale is not None and not sm_scale > 0:
+        raise ValueError(f"sm_scale must be positive (got {sm_scale})")
+    if prefix_len < 0:
+        raise ValueError(f"prefix_len must not be negative (got {prefix_len})")
     pre_ptr, n_pre = 0, 0
     if prefix_len:
         if prefix_pages is None or prefix_pages.dim() != 1:
@@ -703,6 +707,8 @@ def _paged_attention(block, q, index):
 
 def _row_parameter(value, name, dtype, B, index):
     """(pointer, value) of a per-row tensor or of one number for all rows."""
+    if value is None:
+        raise ValueError(f"{name}: expected a number or a tensor")
     if isinstance(value, torch.Tensor):
         if value.dtype != dtype or value.shape != (B,) or not value.is_contiguous():
             raise ValueError(f"{name}: expected a number or a contiguous {dtype} ({B},) tensor")

@@ -149,6 +149,28 @@ def test_generate_is_forward_and_sample():
     assert torch.equal(*same)
 
 
+def test_generate_over_the_fourier_cache():
+    from fourierattention_b200 import DynamicCache, ops
+    model = small_model(False)
+    ids = torch.randint(211, (2, 90), device="cuda", generator=torch.Generator("cuda").manual_seed(8))
+    u = torch.rand(2, 4, device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    path = write_tables(fo.make_splithead_tables(2, 2, 64, 48, seed=3))
+    try:
+        mk = lambda: DynamicCache(make_config(dict(S=4, W=24, M=16, mpe=4096, Hkv=2, steps=8), path))
+        caches = mk(), mk()
+    finally:
+        os.unlink(path)
+    got = model.generate(ids, caches[0], 4, uniform=u, top_k=20)
+    x, want = ids, []
+    with torch.no_grad():
+        for i in range(4):
+            t = ops.sample(model(x, past_key_values=caches[1]).logits[:, -1], u[:, i].contiguous(), top_k=20)
+            want.append(t)
+            x = t[:, None]
+    assert torch.equal(got, torch.stack(want, 1))
+    assert caches[0].get_seq_length(0) == 93
+
+
 def test_paged_decode_step_in_a_graph():
     """A decode step captured once and replayed while lengths and pages move on."""
     from fourierattention_b200 import PagedCache

@@ -355,6 +355,44 @@ def test_attention_page_ids_that_name_no_page(ops):
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
 
 
+def test_attention_without_pages(ops):
+    """A table of no pages, and tokens without sequences."""
+    kp, vp = torch.zeros(2, 2, 2, 16, 64, device="cuda").to(BF)
+    q = torch.randn(3, 4, 64, device="cuda").to(BF)
+    none = torch.zeros((3, 0), dtype=torch.int32, device="cuda")
+    out, lse = ops.paged_attention(q, kp, vp, none, torch.tensor([5, 0, -3], dtype=torch.int32, device="cuda"), return_lse=True)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    kv = torch.randn(3, 2, 64, device="cuda").to(BF)
+    ops.paged_append(kv, kv, kp, vp, none, torch.tensor([5, 0, -3], dtype=torch.int32, device="cuda"), inv_freq(64))
+    assert bool((kp == 0).all()) and bool((vp == 0).all())
+    got = ops.paged_attention(q[:0], kp, vp, none[:0], torch.zeros(0, dtype=torch.int32, device="cuda"))
+    assert got.shape == (0, 4, 64)
+    out = torch.full_like(q, 3.0)
+    ops.paged_attention(q, kp, vp, none[:0], torch.zeros(0, dtype=torch.int32, device="cuda"),
+                        cu_seqlens=torch.zeros(1, dtype=torch.int32, device="cuda"), out=out)
+    assert bool((out == 3).all())
+
+
+def test_attention_shared_pages_and_strided_table(ops):
+    """Sequences that name the same pages, a table that is a view of a wider one."""
+    torch.manual_seed(2)
+    d, ps, n = 128, 32, 90
+    kp, vp, table, _ = make_pages([n], 2, d, ps, HF)
+    k, v = torch.randn(n, 2, d, device="cuda").to(HF), torch.randn(n, 2, d, device="cuda").to(HF)
+    for i in range(3):
+        m = min(ps, n - ps * i)
+        kp[int(table[0, i]), :, :m], vp[int(table[0, i]), :, :m] = k[ps * i:ps * i + m].transpose(0, 1), v[ps * i:ps * i + m].transpose(0, 1)
+    wide = torch.full((4, 9), -5, dtype=torch.int32, device="cuda")
+    wide[:, 2:5] = table[:, :3]
+    q = torch.randn(4, 8, d, device="cuda").to(HF)
+    lens = [90, 1, 64, 33]
+    out = ops.paged_attention(q, kp, vp, wide[:, 2:6], torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    none = torch.zeros(0, 2, d, device="cuda", dtype=HF)
+    o, _, a, e = attend_ref(q, [1] * 4, lens, [k[:x] for x in lens], [v[:x] for x in lens], none, none, d ** -0.5)
+    h = half_step(HF)
+    assert excess((out.double() - o).abs(), h * o.abs() + (h + 2 * e + 2.0 ** -18) * a + 2.0 ** -24) <= 0
+
+
 def test_attention_far_offsets(ops):
     """Pages beyond 2^31 elements, lengths beyond the table."""
     d, ps, hkv = 128, 1024, 8

@@ -93,7 +93,8 @@ def attend_args(**kw):
 @pytest.mark.parametrize("kw", [
     dict(q=_t(2, 8, 64, dtype=F32)), dict(q=_t(2, 8, 64, dtype=HF)), dict(q=_t(3, 8, 64)), dict(q=_t(2, 512)), dict(q=_t(2, 8, 32)),
     dict(k_pages=_t(2, 16, 64)), dict(v_pages=_t(5, 2, 32, 64)), dict(prefix_len=5), dict(prefix_len=5, prefix_pages=_t(1, 1, dtype=torch.int32)),
-    dict(prefix_len=5, prefix_pages=torch.tensor([1])), dict(out=_t(2, 8, 32)), dict(out=_t(2, 8, 64, dtype=HF)), dict(cu_seqlens=_i(0, 1, 2, 3))])
+    dict(prefix_len=5, prefix_pages=torch.tensor([1])), dict(out=_t(2, 8, 32)), dict(out=_t(2, 8, 64, dtype=HF)), dict(cu_seqlens=_i(0, 1, 2, 3)),
+    dict(sm_scale=0.0), dict(sm_scale=-1.0), dict(prefix_len=-1)])
 def test_paged_attention_refuses(ops, kw):
     with pytest.raises(ValueError):
         ops.paged_attention(**attend_args(**kw))
@@ -108,7 +109,8 @@ def sample_args(**kw):
 @pytest.mark.parametrize("kw", [
     dict(logits=_t(3, 100, dtype=torch.float64)), dict(logits=_t(100)), dict(logits=_t(100, 3).T), dict(u=_t(2, dtype=F32)),
     dict(u=_t(3)), dict(temperature=_t(2, dtype=F32)), dict(temperature=_t(3)), dict(top_k=torch.tensor([1, 2, 3])),
-    dict(top_p=_t(3, 1, dtype=F32)), dict(min_p=_t(6, dtype=F32)[::2])])
+    dict(top_p=_t(3, 1, dtype=F32)), dict(min_p=_t(6, dtype=F32)[::2]),
+    dict(temperature=None)])
 def test_sample_refuses(ops, kw):
     with pytest.raises(ValueError):
         ops.sample(**sample_args(**kw))
