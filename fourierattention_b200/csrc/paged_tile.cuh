@@ -4,10 +4,12 @@
 //   S = Q K^T   (tcgen05.mma, both from shared memory, M = N = 128),  P = 2^(S - m) rounded to the cache's type,
 //   O += P V    (tcgen05.mma, P from tensor memory, V as it lies in the page: the MN-major operand).
 // Bound: the tensor pipe (2 x 512 cycles per query tile and key tile at D = 128) and the exponentials (16 per cycle and
-// SM: 1024 cycles), which run side by side: the warps of one query tile work while the other's products run.
-//   warps 0-7, 8-15  softmax of query tile 0 / 1: two threads per row, 64 keys each.  One thread per row with 128 keys
-//                    took 4900 cycles per key tile, bound by the latency of a lone warp per scheduler and tile; four
-//                    warps per scheduler cover it.  The two halves agree through one barrier with a vote.
+// SM: 1024 cycles), which run side by side: the warps of one query tile work while the other's products run.  Reached is
+// 53 % of either (1.03 PFLOP/s with full blocks, 352 us for 403 GFLOP at 1.64 GHz): a query tile's chain of scores, maximum,
+// exponentials and product takes 3350 cycles per key tile.
+//   warps 0-7, 8-15  softmax of query tile 0 / 1: two threads per row, 64 keys each, which agree through one barrier with
+//                    a vote.  Four warps per scheduler cover one another's latencies better than two with 128 keys per
+//                    thread (8 x up to 250 rows of 4 heads over 16384 keys: 489 us against 517, otherwise alike).
 //   warp 16          issues the MMAs and owns tensor memory.  The issuing lane is chosen by elect.sync, descriptors are
 //                    made once: the operands then sit in uniform registers and an MMA takes ~20 cycles to issue; behind
 //                    `lane == 0`, with descriptors made per MMA, it took 100 to 160 and bound the kernel (an MMA of

@@ -21,7 +21,8 @@
 // to 32 neighbouring elements, read four at a time, its groups of four turned by its number so that a walk meets no bank
 // twice) and exchanges partial
 // results through distributed shared memory: every CTA reads all of them and decides alike, one cluster barrier per
-// step.  Bound: latency of those steps for few rows, issue of the float64 exponentials for many.
+// step.  Bound: the latency of those steps (a cluster barrier is ~1500 cycles, a pass over the CTA's elements 4 to 12
+// thousand).  Measured: one row of 128256 34 us, 256 float32 rows 216 us (the row's bytes alone: 20 us).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
