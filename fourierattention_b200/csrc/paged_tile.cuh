@@ -55,8 +55,8 @@ struct PaTile {
     uint32_t tmem;
     int dead;
   };
-  static constexpr int SMEM = QBYTES + ST * SLOT + 3072;
-  static_assert(sizeof(Small) <= 3072, "barriers");
+  static constexpr int SMEM = QBYTES + ST * SLOT + 3 * 1024;
+  static_assert(sizeof(Small) <= 3 * 1024, "barriers");
 };
 
 struct PaTileParams {

@@ -22,7 +22,8 @@
 // twice) and exchanges partial
 // results through distributed shared memory: every CTA reads all of them and decides alike, one cluster barrier per
 // step.  Bound: the latency of those steps (a cluster barrier is ~1500 cycles, a pass over the CTA's elements 4 to 12
-// thousand).  Measured: one row of 128256 34 us, 256 float32 rows 216 us (the row's bytes alone: 20 us).
+// thousand).  Measured: one row of 128256 27 us, 256 float32 rows 214 us (the rows' bytes alone: 20 us).  Everything is inlined:
+// with the state behind a pointer it lived in local memory, and a row took 34 us.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -95,6 +96,12 @@ __device__ __forceinline__ double sa_exp(double z, const double* table) {
   const double e = __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p));
   return z < -700.0 ? 0.0 : e;
 }
+// The bin of a distance from the largest logit: the nearest multiple of 1 / scale, by adding 2^23 (a conversion to an
+// integer takes the slow pipe, which the exponentials need).  Monotone in d; 0 for d = 0 even where scale is infinite.
+__device__ __forceinline__ int sa_bin(float d, float scale) {
+  const float t = d > 0.f ? d * scale : 0.f;
+  return min(SA_BINS - 1, __float_as_int(t + 8388608.f) - 0x4b000000);
+}
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -154,7 +161,8 @@ struct Sampler {
   }
   // f(logit, index, weight) for the elements that `want` takes: first which they are, then their weights, two at a time,
   // so that a warp computes as many as its busiest lane has, not one for every element that some lane has
-  template <typename P, typename F>
+  // (MANY: where most may be wanted).
+  template <bool MANY, typename P, typename F>
   __device__ __forceinline__ void each_weight(P want, F f) {
     for (int r = 0; r < p.rounds; ++r) {
       const int t = r * SA_THREADS + tid, i0 = t << p.ept_log2;
@@ -164,6 +172,19 @@ struct Sampler {
         const int i = base + i0 + 4 * c;
         mask |= ((unsigned)want(v.x, i) | (unsigned)want(v.y, i + 1) << 1 | (unsigned)want(v.z, i + 2) << 2 |
                  (unsigned)want(v.w, i + 3) << 3) << (4 * c);
+      }
+      if (MANY && __reduce_add_sync(0xffffffffu, __popc(mask)) > 16 << p.ept_log2) {
+        // more than half of the warp's elements: all weights, four at a time
+        for (int c = 0; c < 1 << (p.ept_log2 - 2); ++c) {
+          const float4 v = four(t, c);
+          const int i = i0 + 4 * c;
+          const double w0 = weight(v.x), w1 = weight(v.y), w2 = weight(v.z), w3 = weight(v.w);
+          if ((mask >> (4 * c)) & 1) f(v.x, base + i, w0);
+          if ((mask >> (4 * c)) & 2) f(v.y, base + i + 1, w1);
+          if ((mask >> (4 * c)) & 4) f(v.z, base + i + 2, w2);
+          if ((mask >> (4 * c)) & 8) f(v.w, base + i + 3, w3);
+        }
+        continue;
       }
       while (mask) {
         const int a = __ffs(mask) - 1;
@@ -228,7 +249,7 @@ struct Sampler {
   }
 
   // index of the m-th (from 0) element equal to x in the order of the indices
-  __device__ int nth_tie(float x, int m) {
+  __device__ __forceinline__ int nth_tie(float x, int m) {
     int mine = 0;
     each([&](float v, int i) { mine += kept(v, i) && v == x; });
     if (p.rounds == 1) {
@@ -243,7 +264,7 @@ struct Sampler {
     }
     return tie_rounds(x, m);
   }
-  __device__ int tie_locate(float x, int m, int excl, int mine, int round, int wtotal) {
+  __device__ __forceinline__ int tie_locate(float x, int m, int excl, int mine, int round, int wtotal) {
     __syncthreads();
     if (lane == 31) sh.red_n[0][warp] = wtotal;
     if (tid == 0) sh.pick_i = -1;
@@ -268,7 +289,7 @@ struct Sampler {
     return share_pick();
   }
   // the index found by one thread of the cluster, to all
-  __device__ int share_pick() {
+  __device__ __forceinline__ int share_pick() {
     if (tid == 0) sh.x[xb].n[0] = sh.pick_i;
     cl.sync();
     int found = -1;
@@ -277,7 +298,7 @@ struct Sampler {
     return found;
   }
   // several rounds: CTAs hold whole ranges of indices, so the CTA first, then its rounds one by one
-  __device__ int tie_rounds(float x, int m) {
+  __device__ __forceinline__ int tie_rounds(float x, int m) {
     int mine = 0;
     each([&](float v, int i) { mine += kept(v, i) && v == x; });
     mine = __reduce_add_sync(0xffffffffu, mine);
@@ -324,14 +345,14 @@ struct Sampler {
 
   // Shortens the kept head: to its first `k` elements (by_weight false), or to the shortest one whose weight reaches
   // `goal` (by_weight true).  The element it ends with is in [lo, hi].
-  __device__ void shorten(bool by_weight, int k, double goal, float lo, float hi) {
+  __device__ __forceinline__ void shorten(bool by_weight, int k, double goal, float lo, float hi) {
     double near = 0.0;                 // what lies above hi: a number of elements or a weight
     for (int level = 0; level < 256; ++level) {
       // a bin number that never falls with hi - x, whatever the rounding; 0 for hi and the last one for lo, so that
       // every level separates the two
       const float half = hi - lo < INFINITY ? 1.f : 0.5f;
       const float top = half * hi, range = top - half * lo, scale = (float)SA_BINS / range;
-      auto bin_of = [&](float x) { return min(SA_BINS - 1, (int)(fmaf(-half, x, top) * scale)); };
+      auto bin_of = [&](float x) { return sa_bin(fmaf(-half, x, top), scale); };
       const float width = range / (float)SA_BINS / half, c_w = (float)inv_t;
       __syncthreads();
       for (int i = tid; i < SA_BINS; i += SA_THREADS) sh.hist[i] = 0;
@@ -340,8 +361,8 @@ struct Sampler {
         if (!kept(x, i) || x > hi || x < lo) return;
         const int b = bin_of(x);
         // weights relative to the bin's near edge, in steps of 2^-14; a bin may hold 2^18 of the largest
-        const float rel = fminf(0.f, (x - hi + (float)b * width) * c_w);
-        atomicAdd(&sh.hist[b], by_weight ? max(1u, __float2uint_rn(16384.f * __expf(rel))) : 1u);
+        const float rel = fminf(0.f, (x - hi + fmaxf(0.f, (float)b - 0.5f) * width) * c_w);
+        atomicAdd(&sh.hist[b], by_weight ? max(1u, __float_as_uint(fmaf(16384.f, __expf(rel), 8388608.f)) - 0x4b000000u) : 1u);
       });
       cl.sync();
       // two neighbouring bins per thread, over the cluster
@@ -350,8 +371,8 @@ struct Sampler {
       double v0 = (double)h0, v1 = (double)h1;
       if (by_weight) {
         // relative to the weight at hi
-        v0 *= sa_exp((double)(2 * tid * width) * -inv_t, sh.exp2);
-        v1 *= sa_exp((double)((2 * tid + 1) * width) * -inv_t, sh.exp2);
+        v0 *= sa_exp((double)fmaxf(0.f, ((float)(2 * tid) - 0.5f) * width) * -inv_t, sh.exp2);
+        v1 *= sa_exp((double)(((float)(2 * tid) + 0.5f) * width) * -inv_t, sh.exp2);
       }
       double total, pre = block_scan(v0 + v1, total) - (v0 + v1);   // what lies before this thread's bins
       // the histogram counts weights in units of 2^-14 of the weight at hi
@@ -386,7 +407,7 @@ struct Sampler {
           }
         };
         auto want = [&](float x, int i) { return kept(x, i) && x >= lo && (x > hi || bin_of(x) <= b); };
-        if (by_weight) each_weight(want, take);
+        if (by_weight) each_weight<false>(want, take);
         else each([&](float x, int i) {
           if (want(x, i)) take(x, i, 0.0);
         });
@@ -424,7 +445,7 @@ struct Sampler {
   }
 
   // the bin is one value: its first m ties are kept
-  __device__ void cut_ties(float x, bool by_weight, int k, double goal, const SaXchg& o) {
+  __device__ __forceinline__ void cut_ties(float x, bool by_weight, int k, double goal, const SaXchg& o) {
     int m = k - o.n[0];
     if (by_weight) {
       const double w = weight(x);
@@ -448,7 +469,7 @@ struct Sampler {
     return __uint_as_float((u >> 31) ? u : ~(u | 0x80000000u));
   }
   // ascending order of one key per thread, the first n of which count (a bitonic network: within warps by shuffles)
-  __device__ unsigned long long sort_keys(unsigned long long k, int n_all) {
+  __device__ __forceinline__ unsigned long long sort_keys(unsigned long long k, int n_all) {
     int n2 = 32;
     while (n2 < n_all) n2 *= 2;
     for (int len = 2; len <= n2; len *= 2)
@@ -468,7 +489,7 @@ struct Sampler {
     return k;
   }
   // the listed elements of the cluster, one per thread
-  __device__ unsigned long long gather_list() {
+  __device__ __forceinline__ unsigned long long gather_list() {
     static_assert(SA_LIST == SA_THREADS, "an element per thread");
     const int mine = lane < size ? (int)*cl.map_shared_rank(&sh.ln, lane) : 0;
     unsigned long long k = ~0ull;
@@ -483,7 +504,7 @@ struct Sampler {
     return k;
   }
   // running sum of one value per thread, and the sum of all
-  __device__ double block_scan(double v, double& total) {
+  __device__ __forceinline__ double block_scan(double v, double& total) {
     double inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -504,7 +525,7 @@ struct Sampler {
     return pre + inc;
   }
   // cuts the kept head at the k-th of the n listed elements, or at the first where the running sum reaches the goal
-  __device__ void cut_list(int n_all, bool by_weight, int k, double before, double goal) {
+  __device__ __forceinline__ void cut_list(int n_all, bool by_weight, int k, double before, double goal) {
     const unsigned long long key = sort_keys(gather_list(), n_all);
     __syncthreads();
     if (tid == 0) sh.pick = n_all - 1;
@@ -525,10 +546,10 @@ struct Sampler {
   }
 
   // Small top-k: true if the token has been drawn.  `mine` is the largest of the logits this thread has read.
-  __device__ bool draw_short(int row, int k, float mine, float low, float top_p, double min_p, double u) {
+  __device__ __forceinline__ bool draw_short(int row, int k, float mine, float low, float top_p, double min_p, double u) {
     const float half = M - low < INFINITY ? 1.f : 0.5f;
     const float top = half * M, range = top - half * low, scale = (float)SA_BINS / range;
-    auto bin_of = [&](float x) { return min(SA_BINS - 1, (int)(fmaf(-half, x, top) * scale)); };
+    auto bin_of = [&](float x) { return sa_bin(fmaf(-half, x, top), scale); };
     for (int i = tid; i < SA_BINS; i += SA_THREADS) sh.hist[i] = 0;
     if (tid == 0) sh.pick = SA_BINS, sh.ln = 0;
     __syncthreads();
@@ -555,7 +576,7 @@ struct Sampler {
     const int b = sh.pick;
     if (b >= SA_BINS) return false;      // fewer threads with logits than k
     // a border a little below the bin's far edge, whatever the rounding: more elements on the list do no harm
-    const float border = fmaxf(low, (top - ((float)(b + 1) * 1.0001f) / scale) / half);
+    const float border = b == SA_BINS - 1 ? low : fmaxf(low, (top - ((float)b + 0.501f) / scale) / half);
     each([&](float x, int i) {
       if (x >= border) {
         const unsigned slot = atomicAdd(&sh.ln, 1u);
@@ -600,7 +621,7 @@ struct Sampler {
     return true;
   }
 
-  __device__ void run(int row) {
+  __device__ __forceinline__ void run(int row) {
     const T* x = reinterpret_cast<const T*>(p.logits) + (int64_t)row * p.sb;
     xb = 0;
     // The CTA's elements begin on 16 bytes: the row is led in by up to 7 that do not exist (unless the last CTA has no
@@ -703,7 +724,7 @@ struct Sampler {
     if (top_k > 0 && top_k < n_fin) shorten(false, top_k, 0.0, low, M);
     if (top_p < 1.f) {
       double s = 0.0;
-      each_weight([&](float v, int i) { return kept(v, i); }, [&](float, int, double w) { s += w; });
+      each_weight<true>([&](float v, int i) { return kept(v, i); }, [&](float, int, double w) { s += w; });
       exchange(s, 0.0, 0.f, 0.f, 0, 0, o);
       // logits so low that all of them together weigh less than half of what top-p drops are not where it ends
       const double p0 = (double)fmaxf(top_p, 0.f);
@@ -713,7 +734,7 @@ struct Sampler {
     draw(row, u, (double)min_p);
   }
 
-  __device__ void draw(int row, double u, double min_p) {
+  __device__ __forceinline__ void draw(int row, double u, double min_p) {
     double W = 0.0;
     auto mass = [&](int i) -> double {
       const float v = at(i);
@@ -722,15 +743,13 @@ struct Sampler {
       return w >= min_p || v == M ? w : 0.0;
     };
     double mine[SA_MAX_ROUNDS] = {0.0, 0.0, 0.0}, s = 0.0;
-    each_weight([&](float v, int i) { return kept(v, i); },
-                [&](float v, int i, double w) {
-                  const int r = (i - base) >> (p.ept_log2 + 9);
-                  static_assert(SA_THREADS == 512, "2^9 threads");
-                  if (w >= min_p || v == M) {
-#pragma unroll
-                    for (int x = 0; x < SA_MAX_ROUNDS; ++x) mine[x] += x == r ? w : 0.0;
-                  }
-                });
+    each_weight<true>([&](float v, int i) { return kept(v, i); },
+                      [&](float v, int i, double w) {
+                        const int r = (i - base) >> (p.ept_log2 + 9);
+                        static_assert(SA_THREADS == 512, "2^9 threads");
+                        const double x = w >= min_p || v == M ? w : 0.0;
+                        mine[0] += r == 0 ? x : 0.0, mine[1] += r == 1 ? x : 0.0, mine[2] += r == 2 ? x : 0.0;
+                      });
 #pragma unroll
     for (int r = 0; r < SA_MAX_ROUNDS; ++r) s += mine[r];
     // the CTA's sum, and those of the CTAs before it
@@ -791,7 +810,7 @@ struct Sampler {
   }
 
   template <typename F>
-  __device__ void finish(int row, double goal, double own_pre, double W, const double* mine, F mass) {
+  __device__ __forceinline__ void finish(int row, double goal, double own_pre, double W, const double* mine, F mass) {
     unsigned key = (unsigned)sh.pick_i;
     if (key == 0xffffffffu) {
       // rounding at the very end: the last thread with weight
@@ -840,7 +859,7 @@ struct Sampler {
 };
 
 // CTAS: how many share an SM.  Alone a CTA keeps its values in registers (118 instead of 64) and is 7 % faster; two hide
-// each other's waits (256 rows of 128256: 218 us against 306).
+// each other's waits (256 rows of 128256: 214 us against 306).
 template <typename T, int CTAS>
 __global__ void __launch_bounds__(SA_THREADS, CTAS) sample_kernel(const SampleParams p) {
   extern __shared__ float sa_xs[];
