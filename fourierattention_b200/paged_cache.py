@@ -55,7 +55,6 @@ class PagedCache(Cache):
         self._pages: List[List[int]] = [[] for _ in range(batch)]
         self._free: List[int] = list(range(self.num_pages - 1, -1, -1))
         self._plan: Optional[List[int]] = None              # new tokens of the next step, where given
-        self._step: List[int] = [0] * batch                 # new tokens of the current step
         self._prefix_ids: List[int] = []
 
     # -------------------------------------------------------------------------------------------- steps
@@ -88,7 +87,7 @@ class PagedCache(Cache):
                 self._pages[b].append(self._free.pop())
         if sum(grow):
             self._upload_table()
-        self.lengths, self._step = lengths, new
+        self.lengths = lengths
         if all(n == 1 for n in new):
             self.kv_lens.add_(1)
             self.cu_seqlens = None
