@@ -519,8 +519,8 @@ static PaPlan pa_plan(const fa_paged_attn_args_t* a) {
     return r;
   };
   // Blocks that a sequence's own rows fill read the prefix no more often by themselves than packed with others', and the
-  // prefix in front of their own keys saves a launch, the partial results and the merge (8 x up to 250 tokens of 4 heads
-  // per group over 16384 keys: 503 us as two phases); emptier blocks are better packed across the batch.
+  // prefix in front of their own keys saves a launch and partial results (4 heads per group: 8 x up to 250 tokens over
+  // 16384 keys 422 us against 436 as two phases, 4 x up to 1000 over 8192 459 against 551); emptier blocks are better packed across the batch.
   pl.lead = a->prefix_len > 0 && pl.rows_own == PT_ROWS && own >= 3 * PT_ROWS / 4;
   const bool shared = a->prefix_len > 0 && !pl.lead;
   for (int i = 0; i < (shared ? 2 : 1); ++i) {
