@@ -355,6 +355,31 @@ def test_attention_page_ids_that_name_no_page(ops):
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
 
 
+def test_many_sequences(ops):
+    """More sequences than a CTA has threads: every scan over them takes several per thread."""
+    check_attention(ops, [1] * 1500, [(7 * b) % 40 for b in range(1500)], 0, 4, 1, 64, 16, BF)
+    new = [(0, 1, 2, 9)[b % 4] for b in range(900)]
+    check_attention(ops, new, [n + (5 * b) % 30 for b, n in enumerate(new)], 50, 8, 2, 64, 16, HF, pad=2)
+    check_attention(ops, [3 * (b % 30) for b in range(400)], [3 * (b % 30) + b % 7 for b in range(400)], 70, 8, 2, 64, 32, BF)
+    lens = [n + (5 * b) % 30 for b, n in enumerate(new)]
+    kp, vp, table, _ = make_pages(lens, 1, 64, 16, BF)
+    t = sum(new)
+    k, v = torch.randn(t, 1, 64, device="cuda").to(BF), torch.randn(t, 1, 64, device="cuda").to(BF)
+    f = inv_freq(64)
+    ops.paged_append(k, v, kp, vp, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), f,
+                     cu_seqlens=torch.tensor([0] + np.cumsum(new).tolist(), dtype=torch.int32, device="cuda"))
+    at = torch.cat([torch.arange(l - n, l) for l, n in zip(lens, new)]).cuda()
+    seq = torch.repeat_interleave(torch.arange(900), torch.tensor(new)).cuda()
+    page = table[seq, at // 16].long()
+    assert torch.equal(vp[page, 0, at % 16], v[:, 0])
+    ref = rope_ref(k, None, 0, at, f)
+    close(kp[page, 0, at % 16], ref[:, 0], BF, ref[:, 0].abs().amax(-1, keepdim=True) + 1)
+    assert int((~vp.isnan()).sum()) == t * 64
+    x, u = torch.randn(3000, 257, device="cuda"), torch.rand(3000, device="cuda")
+    check_sample(ops, x, u, top_k=30, top_p=0.9)
+    check_sample(ops, x, u, top_p=0.7, min_p=0.01)
+
+
 def test_attention_without_pages(ops):
     """A table of no pages, and tokens without sequences."""
     kp, vp = torch.zeros(2, 2, 2, 16, 64, device="cuda").to(BF)
