@@ -574,7 +574,10 @@ struct Sampler {
     else if (v1 > 0 && pre + v0 + v1 >= k) atomicMin(&sh.pick, 2 * tid + 1);
     __syncthreads();
     const int b = sh.pick;
-    if (b >= SA_BINS) return false;      // fewer threads with logits than k
+    if (b >= SA_BINS) {                  // fewer threads with logits than k
+      cl.sync();                         // the histograms are written anew
+      return false;
+    }
     // a border a little below the bin's far edge, whatever the rounding: more elements on the list do no harm
     const float border = b == SA_BINS - 1 ? low : fmaxf(low, (top - ((float)b + 0.501f) / scale) / half);
     each([&](float x, int i) {

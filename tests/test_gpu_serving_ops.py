@@ -599,3 +599,22 @@ def test_sample_strides_streams_graphs(ops):
     torch.cuda.synchronize()
     assert torch.equal(c, ops.sample(x, u, top_k=20, top_p=0.9))
     assert ops.sample(x[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.parametrize("B,V", [(1, 128256), (5, 128256), (20, 128256), (150, 20000), (3, 4100)])
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("run", [300, 1000])
+def test_sample_masked_to_neighbours(ops, B, V, dtype, run):
+    """Long rows masked to a run of neighbouring tokens, as a grammar does: few threads hold a logit that can be drawn,
+    fewer than top-k wants (a thread reads 4 or 8 neighbours at once), in clusters of 1 to 8 CTAs."""
+    torch.manual_seed(B + run)
+    x = torch.full((B, V), -math.inf, device="cuda", dtype=dtype)
+    for b in range(B):
+        at = (997 * b) % (V - run)
+        x[b, at:at + run] = (2 * torch.randn(run, device="cuda")).to(dtype)
+    u = torch.rand(B, device="cuda")
+    for k in (run // 6, run // 3, run - 1, run, run + 1):
+        if k <= 512:
+            check_sample(ops, x, u, top_k=k)
+        check_sample(ops, x, u, top_k=k, top_p=0.8, min_p=0.001)
+    check_sample(ops, x, u, top_p=0.9)
