@@ -177,10 +177,10 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int rr = min(nt * 8 + c2 + j, n_rows - 1);
-        lim[nt][j] = p.prefix_len > 0 ? u.s.L : min(u.s.L, u.s.L - u.s.n + (row0 + rr) / c.G + 1);
+        lim[nt][j] = p.prefix_len > 0 ? u.s.L : min(u.s.L, u.s.len - u.s.n + (row0 + rr) / c.G + 1);
       }
     }
-    const int lim0 = p.prefix_len > 0 ? u.s.L : u.s.L - u.s.n + row0 / c.G + 1;     // the first row sees least
+    const int lim0 = p.prefix_len > 0 ? u.s.L : min(u.s.L, u.s.len - u.s.n + row0 / c.G + 1);     // the first row sees least
     float o[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {

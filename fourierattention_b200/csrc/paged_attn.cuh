@@ -44,7 +44,7 @@ struct PaCommon {
 };
 
 struct PaSeq {
-  int t0, n, L;              // first new token, number of new tokens, number of keys
+  int t0, n, L, len;         // first new token, number of new tokens, number of keys that have a page, length
 };
 
 __device__ __forceinline__ PaSeq pa_seq(const PaCommon& c, const PaPhase& p, int b) {
@@ -52,14 +52,16 @@ __device__ __forceinline__ PaSeq pa_seq(const PaCommon& c, const PaPhase& p, int
   if (p.prefix_len > 0) {
     s.t0 = 0;
     s.n = c.cu ? max(0, min(c.tokens, c.cu[c.B])) : c.tokens;
-    s.L = p.prefix_len;
+    s.L = s.len = p.prefix_len;
     return s;
   }
   int t0 = b, t1 = b + 1;
   if (c.cu) t0 = c.cu[b], t1 = c.cu[b + 1];
   s.t0 = max(0, min(t0, c.tokens));
   s.n = max(0, min(t1, c.tokens) - s.t0);
-  s.L = (int)max(0LL, min((long long)c.kv_lens[b], (long long)p.max_pages * c.page_size));
+  // a token's place counts from the length as it is; keys behind the table do not exist
+  s.len = max(0, c.kv_lens[b]);
+  s.L = (int)min((long long)s.len, (long long)p.max_pages * c.page_size);
   return s;
 }
 __device__ __forceinline__ int pa_seqs(const PaCommon& c, const PaPhase& p) { return p.prefix_len > 0 ? 1 : c.B; }
@@ -70,7 +72,7 @@ __device__ __forceinline__ int pa_blocks(const PaCommon& c, const PaPhase& p, co
 __device__ __forceinline__ int pa_limit(const PaCommon& c, const PaPhase& p, const PaSeq& s, int rb) {
   if (p.prefix_len > 0) return s.L;
   const int last = min(s.n * c.G, (rb + 1) << p.rows_log2) - 1;
-  return max(0, min(s.L, s.L - s.n + (int)((unsigned)last / (unsigned)c.G) + 1));
+  return max(0, min(s.L, s.len - s.n + (int)((unsigned)last / (unsigned)c.G) + 1));
 }
 __device__ __forceinline__ int pa_tiles(int limit) { return (limit + PA_TILE - 1) / PA_TILE; }
 // tiles of a unit whose rows see `limit` keys; those of the lead come first, in tiles of their own

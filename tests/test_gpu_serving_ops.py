@@ -618,3 +618,35 @@ def test_sample_masked_to_neighbours(ops, B, V, dtype, run):
             check_sample(ops, x, u, top_k=k)
         check_sample(ops, x, u, top_k=k, top_p=0.8, min_p=0.001)
     check_sample(ops, x, u, top_p=0.9)
+
+
+@pytest.mark.parametrize("new", [2, 3, 40, 60])
+@pytest.mark.parametrize("prefix", [0, 100])
+@pytest.mark.parametrize("past", [0, 1, 35, 2 ** 31 - 1 - 112])
+def test_attention_lengths_behind_the_table(ops, new, prefix, past):
+    """Several new tokens whose sequence is longer than its table: the keys behind the table do not exist, and each token
+    sees those before it that do, counted from the length as given."""
+    torch.manual_seed(new + prefix)
+    d, ps, hkv, hq, cap = 64, 16, 2, 8, 112
+    kp, vp, table, _ = make_pages([cap, 30, prefix], hkv, d, ps, BF)
+    pre, table = table[2, :-(-prefix // ps)].contiguous(), table[:2].contiguous()
+    keys, values = [], []
+    for ids, n in ((pre, prefix), (table[0], cap), (table[1], 30)):
+        k, v = torch.randn(n, hkv, d, device="cuda").to(BF), torch.randn(n, hkv, d, device="cuda").to(BF)
+        for j0 in range(0, n, ps):
+            m = min(ps, n - j0)
+            kp[int(ids[j0 // ps]), :, :m], vp[int(ids[j0 // ps]), :, :m] = k[j0:j0 + m].transpose(0, 1), v[j0:j0 + m].transpose(0, 1)
+        keys.append(k)
+        values.append(v)
+    lens, news = [cap + past, 30], [new, new]
+    q = (2 * torch.randn(2 * new, hq, d, device="cuda")).to(BF)
+    cu = torch.tensor([0, new, 2 * new], dtype=torch.int32, device="cuda")
+    out, lse = ops.paged_attention(q, kp, vp, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), cu_seqlens=cu,
+                                   prefix_pages=pre if prefix else None, prefix_len=prefix, return_lse=True)
+    o, rl, a, e = attend_ref(q, news, lens, keys[1:], values[1:], keys[0], values[0], d ** -0.5)
+    h = half_step(BF)
+    assert excess((out.double() - o).abs(), h * o.abs() + (h + 2 * e + 2.0 ** -18) * a + 2.0 ** -24) <= 0
+    rl, e = rl[..., 0], e[..., 0]
+    some = rl > -math.inf
+    assert excess((lse.double() - rl)[some].abs(), (e + 2.0 ** -18 + 2.0 ** -22 * rl.abs())[some]) <= 0
+    assert bool((lse[~some] == -math.inf).all()) and bool((out[~some] == 0).all())
