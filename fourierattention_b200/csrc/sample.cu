@@ -235,8 +235,9 @@ struct Sampler {
     out.n[0] = __shfl_sync(0xffffffffu, out.n[0], 0), out.n[1] = __shfl_sync(0xffffffffu, out.n[1], 0);
     xb ^= 1;
   }
-  // this thread's two bins of the histogram, over the cluster
-  __device__ __forceinline__ void read_bins(unsigned& a, unsigned& b) {
+  // this thread's two bins of the histogram, over the cluster: a CTA's count of up to 49152 x 2^14 fits 32 bits, the sum
+  // of eight does not
+  __device__ __forceinline__ void read_bins(unsigned long long& a, unsigned long long& b) {
     uint2 h[SA_MAX_CLUSTER];
 #pragma unroll
     for (int r = 0; r < SA_MAX_CLUSTER; ++r) {
@@ -360,13 +361,13 @@ struct Sampler {
       each([&](float x, int i) {
         if (!kept(x, i) || x > hi || x < lo) return;
         const int b = bin_of(x);
-        // weights relative to the bin's near edge, in steps of 2^-14; a bin may hold 2^18 of the largest
+        // weights relative to the bin's near edge, in steps of 2^-14
         const float rel = fminf(0.f, (x - hi + fmaxf(0.f, (float)b - 0.5f) * width) * c_w);
         atomicAdd(&sh.hist[b], by_weight ? max(1u, __float_as_uint(fmaf(16384.f, __expf(rel), 8388608.f)) - 0x4b000000u) : 1u);
       });
       cl.sync();
       // two neighbouring bins per thread, over the cluster
-      unsigned h0, h1;
+      unsigned long long h0, h1;
       read_bins(h0, h1);
       double v0 = (double)h0, v1 = (double)h1;
       if (by_weight) {
@@ -555,7 +556,7 @@ struct Sampler {
     __syncthreads();
     if (mine > -INFINITY) atomicAdd(&sh.hist[bin_of(mine)], 1u);
     cl.sync();
-    unsigned h0, h1;
+    unsigned long long h0, h1;
     read_bins(h0, h1);
     const int v0 = (int)h0, v1 = (int)h1;
     int pre = v0 + v1;

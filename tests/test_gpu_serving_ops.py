@@ -650,3 +650,33 @@ def test_attention_lengths_behind_the_table(ops, new, prefix, past):
     some = rl > -math.inf
     assert excess((lse.double() - rl)[some].abs(), (e + 2.0 ** -18 + 2.0 ** -22 * rl.abs())[some]) <= 0
     assert bool((lse[~some] == -math.inf).all()) and bool((out[~some] == 0).all())
+
+
+def _time(f, n=5):
+    best = math.inf
+    for _ in range(n):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+@pytest.mark.parametrize("V", [262144, 393216])
+def test_sample_large_vocabulary_of_equal_logits(ops, V):
+    """2^18 equal weights fill 32 bits of a bin's count.  The proposal of a bin still names the right one: a wrong one is
+    put right bin by bin, over a thousand passes over the row, where a proposal takes a few."""
+    u = torch.tensor([0.0, 0.37, 0.93], device="cuda")
+    x = torch.zeros(3, V, device="cuda", dtype=BF)
+    x[:, 262144:] = -9.0                                        # exactly 2^18 of the largest
+    check_sample(ops, x, u, top_p=0.5)
+    x[:, 5] = -1.0
+    check_sample(ops, x, u, top_p=0.25)
+    check_sample(ops, x, u, top_p=0.75, min_p=0.5)
+    x[:, 5] = 0.0
+    spread = torch.randn(3, V, device="cuda").to(BF)
+    ops.sample(spread, u, top_p=0.5)
+    # the same number of passes as any other row, within a factor that a thousand passes would exceed by far
+    assert _time(lambda: ops.sample(x, u, top_p=0.5)) < 10 * _time(lambda: ops.sample(spread, u, top_p=0.5))
