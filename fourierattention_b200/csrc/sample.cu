@@ -603,7 +603,7 @@ struct Sampler {
     const double w = tid < k ? weight(key_value(key)) : 0.0;
     double total, kept_sum;
     const double inc = block_scan(w, total);
-    const bool keep = tid == 0 || (tid < k && w >= min_p && (top_p >= 1.f || inc - w < (double)fmaxf(top_p, 0.f) * total));
+    const bool keep = tid == 0 || (tid < k && w >= min_p && (top_p >= 1.f || inc - w < (double)top_p * total));
     const int n_keep = __syncthreads_count(keep);      // a head of the order, as each of the three is
     // the kept ones in the order of their indices
     sh.gw[tid] = tid < n_keep ? w : 0.0;
@@ -638,9 +638,13 @@ struct Sampler {
     n = max(0, min(p.V - base, p.slice));
     if (tid < 64) sh.exp2[tid] = exp2((double)tid / 64.0);
     const float temperature = p.temperature ? p.temperature[row] : p.temperature0;
-    const float top_p = p.top_p ? p.top_p[row] : p.top_p0;
-    const float min_p = p.min_p ? p.min_p[row] : p.min_p0;
+    // a NaN filter is off; min_p above 1 leaves the largest logit alone, as top_k = 1 does
+    float top_p = p.top_p ? p.top_p[row] : p.top_p0;
+    top_p = top_p < 1.f ? fmaxf(top_p, 0.f) : 1.f;
+    float min_p = p.min_p ? p.min_p[row] : p.min_p0;
+    min_p = min_p > 0.f ? min_p : 0.f;
     int top_k = p.top_k ? p.top_k[row] : p.top_k0;
+    if (min_p > 1.f) top_k = 1;
     // ---- the row, once ------------------------------------------------------------------------------------------
     float mn = INFINITY, mx = -INFINITY;
     int fin = 0;
@@ -731,7 +735,7 @@ struct Sampler {
       each_weight<true>([&](float v, int i) { return kept(v, i); }, [&](float, int, double w) { s += w; });
       exchange(s, 0.0, 0.f, 0.f, 0, 0, o);
       // logits so low that all of them together weigh less than half of what top-p drops are not where it ends
-      const double p0 = (double)fmaxf(top_p, 0.f);
+      const double p0 = (double)top_p;
       const float from = (float)((double)M + log(0.5 * (1.0 - p0) * o.s[0] / (double)n_fin) / inv_t);
       shorten(true, 0, p0 * o.s[0], fmaxf(kx > -INFINITY ? kx : low, fminf(from, M)), M);
     }

@@ -364,10 +364,11 @@ int fa_paged_attn(const fa_paged_attn_args_t* args_host, fa_stream_t stream);
 /* One token per row of logits (B, V), V <= 393216.  Weights w_i = exp((x_i - max x) / temperature), in the order
  * "larger logit first, lower index first among equals"; kept are the first top_k of them (top_k <= 0: all), of those
  * the shortest head whose weight reaches top_p times theirs (top_p >= 1: all), of those the ones of at least min_p
- * times the largest.  The token is the first index whose running sum of kept weights (by index) exceeds u times their
- * sum, 0 <= u < 1; logprob (or null) is the logarithm of its share.  temperature <= 0 takes the largest logit.  A NaN
- * logit is never drawn; logits of +infinity share the probability; a row without a logit above -infinity gives
- * token -1, logprob -infinity.  Every parameter is a (B) device array or, where that is null, the value next to it.
+ * times the largest (the first one always).  The token is the first index whose running sum of kept weights (by index)
+ * exceeds u times their sum, 0 <= u < 1; logprob (or null) is the logarithm of its share.  A temperature not above 0
+ * takes the largest logit, a NaN top_p or min_p filters nothing.  A NaN logit is never drawn; logits of +infinity share
+ * the probability; a row without a logit above -infinity gives token -1, logprob -infinity.  Every parameter is a (B)
+ * device array or, where that is null, the value next to it.
  * Sums that decide are taken in float64 in a fixed order. */
 int fa_sample(const void* logits, int dtype, int B, int V, int64_t logits_sb, const float* u, const float* temperature,
               float temperature0, const int32_t* top_k, int top_k0, const float* top_p, float top_p0, const float* min_p,

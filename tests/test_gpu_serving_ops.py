@@ -680,3 +680,28 @@ def test_sample_large_vocabulary_of_equal_logits(ops, V):
     ops.sample(spread, u, top_p=0.5)
     # the same number of passes as any other row, within a factor that a thousand passes would exceed by far
     assert _time(lambda: ops.sample(x, u, top_p=0.5)) < 10 * _time(lambda: ops.sample(spread, u, top_p=0.5))
+
+
+@pytest.mark.parametrize("V", [64, 30000, 128256])
+@pytest.mark.parametrize("top_k", [0, 40, 20000])
+def test_sample_odd_filter_values(ops, V, top_k):
+    """NaN filters are off and min_p above 1 keeps the first of the largest logits, whichever way a row is searched."""
+    torch.manual_seed(V)
+    B = 6
+    x = torch.randn(B, V, device="cuda").to(BF)
+    x[:, V // 2:V // 2 + 9] = 8.0                               # nine largest
+    u = torch.tensor([0.0, 0.2, 0.4, 0.6, 0.8, 0.99], device="cuda")
+    full = lambda v: torch.full((B,), v, device="cuda")
+    nan = math.nan
+    off = ops.sample(x, u, top_k=top_k, return_logprob=True)
+    for kw in (dict(top_p=full(nan)), dict(min_p=full(nan)), dict(top_p=full(nan), min_p=full(nan)), dict(min_p=full(-1.0)),
+               dict(top_p=full(math.inf))):
+        got = ops.sample(x, u, top_k=top_k, return_logprob=True, **kw)
+        assert torch.equal(got[0], off[0]) and torch.equal(got[1], off[1]), kw
+    assert torch.equal(ops.sample(x, u, top_k=top_k, top_p=full(-3.0)), ops.sample(x, u, top_k=top_k, top_p=0.0))
+    for kw in (dict(min_p=1.5), dict(min_p=full(1.5)), dict(min_p=full(math.inf), top_p=0.9)):
+        token, logprob = ops.sample(x, u, top_k=top_k, return_logprob=True, **kw)
+        assert token.tolist() == [V // 2] * B and bool((logprob == 0).all()), kw
+        check_sample(ops, x, u, top_k=top_k, **kw)
+    check_sample(ops, x, u, top_k=top_k, min_p=1.0)             # all nine
+    assert torch.equal(ops.sample(x, u, temperature=full(nan)), ops.sample(x, u, temperature=0.0))
