@@ -714,6 +714,8 @@ def _row_parameter(value, name, dtype, B, index):
             raise ValueError(f"{name}: expected a number or a contiguous {dtype} ({B},) tensor")
         _on(index, value)
         return value.data_ptr(), 0
+    if value != value or (dtype == torch.int32 and not (hasattr(value, "__index__") and -2 ** 31 <= value < 2 ** 31)):
+        raise ValueError(f"{name}: expected {'a 32-bit integer' if dtype == torch.int32 else 'a number'}, got {value!r}")
     return None, value
 
 
@@ -721,7 +723,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_log
     """Draws one token per row of ``logits`` (B, V), float32, float16 or bfloat16, V <= 393216, with the uniform numbers
     ``u`` (B,) float32 in [0, 1).  Temperature is applied first (0: the largest logit), then top-k (0: off), top-p on
     what top-k kept (1: off), min-p relative to the largest probability (0: off); each is a number or a (B,) tensor
-    (float32, ``top_k`` int32).  Among equal logits the lower index counts as larger.  The token is the first index at
+    (float32, ``top_k`` int32).  A NaN in a tensor of filters turns that one off; as a number it is refused.  Among equal logits the lower index counts as larger.  The token is the first index at
     which the running sum of kept probabilities exceeds u.  Returns int64 tokens, with ``return_logprob`` also the
     float32 logarithm of the probability each had in the kept distribution.  NaN logits are never drawn; a row without a
     logit above -infinity gives token -1."""

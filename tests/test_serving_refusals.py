@@ -179,3 +179,11 @@ def test_library_refuses(ops):
                                               m0=0.0, tok=4096, lp=None, st=None), **kw}.values())
     assert one(dt=3) == -3 and one(V=0) == -2 and one(B=-1) == -2 and one(V=393217) == -5 and one(x=None) == -1
     assert one(u=None) == -1 and one(tok=None) == -1 and one(B=0, x=None) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(top_k=2 ** 31), dict(top_k=2 ** 32 + 5), dict(top_k=-2 ** 31 - 1), dict(top_k=2.5),
+                                dict(temperature=float("nan")), dict(top_p=float("nan")), dict(min_p=float("nan"))])
+def test_sample_refuses_numbers(ops, kw):
+    """A top_k that does not fit its 32 bits would be another one, a NaN is no setting at all."""
+    with pytest.raises(ValueError, match=next(iter(kw))):
+        ops.sample(**sample_args(**kw))
