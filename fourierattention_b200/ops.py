@@ -629,6 +629,8 @@ def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, inv_freq, cu_seqle
         if qs[0] != tokens or qs[2] != D:
             raise ValueError("q and k must have the same tokens and head dimension")
         _like(q_out, "q_out", qs, dtype)
+    elif q_out is not None:
+        raise ValueError("q_out is given without q")
     pos_ptr, wide = 0, 0
     if positions is not None:
         wide, pos_ptr = _positions64(positions, tokens), positions.data_ptr()

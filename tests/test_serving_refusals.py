@@ -187,3 +187,9 @@ def test_sample_refuses_numbers(ops, kw):
     """A top_k that does not fit its 32 bits would be another one, a NaN is no setting at all."""
     with pytest.raises(ValueError, match=next(iter(kw))):
         ops.sample(**sample_args(**kw))
+
+
+def test_paged_append_refuses_an_output_without_queries(ops):
+    """It would come back unwritten."""
+    with pytest.raises(ValueError, match="q_out"):
+        ops.paged_append(**append_args(q_out=_t(2, 8, 64)))
