@@ -113,11 +113,13 @@ class PagedCache(Cache):
                                    prefix_pages=self.prefix_pages, prefix_len=self.prefix_len, sm_scale=sm_scale)
 
     def last_rows(self, hidden):
-        """The hidden state of the last new token of every sequence, (batch, 1, hidden)."""
+        """The hidden state of the last new token of every sequence, (batch, 1, hidden); zeros for one without new tokens in
+        the step."""
         if self.cu_seqlens is None:
             return hidden.reshape(self.batch, 1, -1)
         rows = hidden.reshape(-1, hidden.shape[-1])
-        return rows[(self.cu_seqlens[1:].long() - 1).clamp(min=0)][:, None]
+        end, idle = self.cu_seqlens[1:].long(), self.cu_seqlens[1:] == self.cu_seqlens[:-1]
+        return rows[(end - 1).clamp(min=0)].masked_fill(idle[:, None], 0)[:, None]
 
     # -------------------------------------------------------------------------------------------- sequences
     def share_prefix(self, sequence: int = 0):

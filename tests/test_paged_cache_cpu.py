@@ -87,3 +87,19 @@ def test_prefix(PagedCache):
     c.begin_step(1, 2)
     with pytest.raises(RuntimeError, match="empty"):
         c.share_prefix(0)
+
+
+@pytest.mark.parametrize("new", [[5, 0, 3], [0, 2, 0], [0, 0, 1], [2, 1, 0]])
+def test_last_rows_of_idle_sequences(PagedCache, new):
+    """A sequence without new tokens has no last row: it gets zeros, not a neighbour's (nor its NaN)."""
+    c = make(PagedCache)
+    c.plan(new)
+    c.begin_step(1, sum(new))
+    h = torch.arange(1.0, 1 + 2 * sum(new)).view(1, -1, 2)
+    h[0, 0, 0] = float("nan")
+    got, at = c.last_rows(h), 0
+    assert tuple(got.shape) == (3, 1, 2)
+    for b, n in enumerate(new):
+        at += n
+        want = h[0, at - 1] if n else torch.zeros(2)
+        assert torch.equal(got[b, 0].nan_to_num(-1.0), want.nan_to_num(-1.0))
