@@ -282,8 +282,11 @@ class LlamaForCausalLM(nn.Module):
         """Runs the prompt (``input_ids`` as :meth:`forward` takes them) and draws ``max_new_tokens`` tokens per sequence
         with ``ops.sample`` (its parameters: numbers or one value per sequence; ``temperature=0`` is greedy).
         ``uniform``: (batch, max_new_tokens) float32 in [0, 1), drawn with ``generator`` if not given.  Tokens behind
-        ``eos_token_id`` are ``eos_token_id``.  Returns (batch, max_new_tokens) int64; the last token drawn is not in the
-        cache yet."""
+        ``eos_token_id`` are ``eos_token_id``.  A planned prompt of a ``PagedCache`` has new tokens of every sequence: there
+        is nothing to draw from for one without.  Returns (batch, max_new_tokens) int64; the last token drawn is not in
+        the cache yet."""
+        if isinstance(past_key_values, PagedCache) and 0 in (past_key_values.planned or ()):
+            raise ValueError(f"generate: sequences without new tokens in the plan {past_key_values.planned}")
         tokens, done = [], None
         for i in range(max_new_tokens):
             logits = self(input_ids, past_key_values=past_key_values).logits[:, -1]

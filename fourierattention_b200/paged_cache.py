@@ -66,6 +66,11 @@ class PagedCache(Cache):
             raise ValueError(f"plan: {self.batch} numbers of new tokens are wanted, not all of them 0")
         self._plan = new_tokens
 
+    @property
+    def planned(self) -> Optional[List[int]]:
+        """New tokens of every sequence in the next step, where :meth:`plan` gave them."""
+        return self._plan
+
     def begin_step(self, rows: int, tokens: int):
         """Makes room for the new tokens of a model call on ``(rows, tokens)`` input ids."""
         new = self._plan
