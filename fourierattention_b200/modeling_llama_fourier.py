@@ -270,6 +270,11 @@ class LlamaForCausalLM(nn.Module):
                     m.bias.data.zero_()
 
     def forward(self, input_ids, past_key_values=None, use_cache=True, num_logits_to_keep: int = 1, **kwargs):
+        if isinstance(past_key_values, PagedCache):
+            packed = past_key_values.planned is not None and past_key_values.batch > 1
+            if packed and not (num_logits_to_keep in (0, 1) or num_logits_to_keep >= input_ids.shape[1]):
+                raise ValueError(f"num_logits_to_keep={num_logits_to_keep} of packed tokens: the rows would be of the last "
+                                 "sequences only; 1 gives every sequence's last token, 0 all rows")
         h = self.model(input_ids, past_key_values=past_key_values)
         if isinstance(past_key_values, PagedCache) and num_logits_to_keep == 1:
             h = past_key_values.last_rows(h)                 # of every sequence, packed or not

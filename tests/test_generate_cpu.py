@@ -32,3 +32,29 @@ def test_generate_refuses_idle_sequences(pkg, plan):
     with pytest.raises(ValueError, match="without new tokens"):
         small(pkg).generate(torch.zeros(1, 8, dtype=torch.int64), cache, 2)
     assert cache.lengths == [0, 0, 0] and cache.planned == plan
+
+
+@pytest.mark.parametrize("keep", [2, 7])
+def test_packed_logits_are_not_cut_across_sequences(pkg, keep):
+    """The last rows of packed tokens are those of the last sequences, not the last ones of each."""
+    cache, ids = paged(pkg), torch.zeros(1, 8, dtype=torch.int64)
+    cache.plan([4, 1, 3])
+    with pytest.raises(ValueError, match="num_logits_to_keep"):
+        small(pkg)(ids, past_key_values=cache, num_logits_to_keep=keep)
+    assert cache.lengths == [0, 0, 0] and cache.planned == [4, 1, 3]
+
+
+@pytest.mark.parametrize("keep,rows", [(0, 8), (1, 3), (8, 8), (20, 8)])
+def test_packed_logits(pkg, keep, rows, monkeypatch):
+    """All rows, or the last one of every sequence."""
+    model, cache = small(pkg), paged(pkg)
+    cache.plan([4, 1, 3])
+    hidden = torch.randn(1, 8, 64)
+
+    def layers(ids, past_key_values):
+        past_key_values.begin_step(*ids.shape)
+        return hidden
+    monkeypatch.setattr(model.model, "forward", layers)
+    logits = model(torch.zeros(1, 8, dtype=torch.int64), past_key_values=cache, num_logits_to_keep=keep).logits
+    want = model.lm_head(hidden[0] if rows == 8 else hidden[0, [3, 4, 7]])
+    torch.testing.assert_close(logits.reshape(rows, -1), want)
