@@ -290,6 +290,8 @@ class LlamaForCausalLM(nn.Module):
         ``eos_token_id`` are ``eos_token_id``.  A planned prompt of a ``PagedCache`` has new tokens of every sequence: there
         is nothing to draw from for one without.  Returns (batch, max_new_tokens) int64; the last token drawn is not in
         the cache yet."""
+        if past_key_values is None and max_new_tokens > 1:
+            raise ValueError("generate: more than one token needs a cache")
         if isinstance(past_key_values, PagedCache) and 0 in (past_key_values.planned or ()):
             raise ValueError(f"generate: sequences without new tokens in the plan {past_key_values.planned}")
         tokens, done = [], None

@@ -58,3 +58,9 @@ def test_packed_logits(pkg, keep, rows, monkeypatch):
     logits = model(torch.zeros(1, 8, dtype=torch.int64), past_key_values=cache, num_logits_to_keep=keep).logits
     want = model.lm_head(hidden[0] if rows == 8 else hidden[0, [3, 4, 7]])
     torch.testing.assert_close(logits.reshape(rows, -1), want)
+
+
+def test_generate_needs_a_cache(pkg):
+    """Without one, every token after the first would be drawn without its context."""
+    with pytest.raises(ValueError, match="cache"):
+        small(pkg).generate(torch.zeros(1, 4, dtype=torch.int64), None, 2)
