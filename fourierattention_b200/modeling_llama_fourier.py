@@ -287,7 +287,8 @@ class LlamaForCausalLM(nn.Module):
         """Runs the prompt (``input_ids`` as :meth:`forward` takes them) and draws ``max_new_tokens`` tokens per sequence
         with ``ops.sample`` (its parameters: numbers or one value per sequence; ``temperature=0`` is greedy).
         ``uniform``: (batch, max_new_tokens) float32 in [0, 1), drawn with ``generator`` if not given.  Tokens behind
-        ``eos_token_id`` are ``eos_token_id``.  A planned prompt of a ``PagedCache`` has new tokens of every sequence: there
+        ``eos_token_id`` are ``eos_token_id``.  A sequence whose logits hold nothing to draw (all NaN or -infinity) gets -1
+        and goes on with token 0.  A planned prompt of a ``PagedCache`` has new tokens of every sequence: there
         is nothing to draw from for one without.  Returns (batch, max_new_tokens) int64; the last token drawn is not in
         the cache yet."""
         if past_key_values is None and max_new_tokens > 1:
@@ -306,5 +307,5 @@ class LlamaForCausalLM(nn.Module):
                     token = torch.where(done, eos_token_id, token)
                 done = token == eos_token_id
             tokens.append(token)
-            input_ids = token[:, None]
+            input_ids = token.clamp(min=0)[:, None]          # -1 (nothing to draw) is no row of the embedding
         return torch.stack(tokens, dim=1) if tokens else torch.empty((0, 0), dtype=torch.int64, device=input_ids.device)

@@ -64,3 +64,29 @@ def test_generate_needs_a_cache(pkg):
     """Without one, every token after the first would be drawn without its context."""
     with pytest.raises(ValueError, match="cache"):
         small(pkg).generate(torch.zeros(1, 4, dtype=torch.int64), None, 2)
+
+
+class Recorder:
+    """Stands for the model's forward and for the sampler: what the model is called with, and the given tokens in turn."""
+
+    def __init__(self, pkg, monkeypatch, tokens):
+        self.model, self.seen, self.tokens = small(pkg), [], [torch.tensor(t) for t in tokens]
+        monkeypatch.setattr(self.model, "forward", self.forward)
+        monkeypatch.setattr(pkg.ops, "sample", lambda logits, u, **kw: self.tokens[len(self.seen) - 1])
+
+    def forward(self, input_ids, past_key_values):
+        self.seen.append(input_ids.tolist())
+        return SimpleNamespace(logits=torch.zeros(input_ids.shape[0], 1, 11))
+
+
+@pytest.mark.parametrize("eos", [None, 5, -1])
+def test_generate_never_embeds_what_was_not_drawn(pkg, monkeypatch, eos):
+    """-1, for a row without anything to draw from, is returned and not looked up."""
+    r = Recorder(pkg, monkeypatch, [[3, -1], [5, -1], [-1, 2], [4, 4]])
+    got = r.model.generate(torch.tensor([[1, 2], [3, 4]]), paged(pkg, 2), 4, eos_token_id=eos)
+    assert tuple(got.shape) == (2, 4) and got[:, 0].tolist() == [3, -1]
+    assert r.seen[0] == [[1, 2], [3, 4]] and all(t >= 0 for step in r.seen for row in step for t in row)
+    if eos is None:
+        assert got.tolist() == [[3, 5, -1, 4], [-1, -1, 2, 4]] and r.seen[1:] == [[[3], [0]], [[5], [0]], [[0], [2]]]
+    if eos == 5:
+        assert got[0].tolist() == [3, 5, 5, 5]
