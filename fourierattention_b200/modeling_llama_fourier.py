@@ -291,6 +291,8 @@ class LlamaForCausalLM(nn.Module):
         and goes on with token 0.  A planned prompt of a ``PagedCache`` has new tokens of every sequence: there
         is nothing to draw from for one without.  Returns (batch, max_new_tokens) int64; the last token drawn is not in
         the cache yet."""
+        if max_new_tokens < 0:
+            raise ValueError(f"generate: {max_new_tokens} tokens")
         if past_key_values is None and max_new_tokens > 1:
             raise ValueError("generate: more than one token needs a cache")
         if isinstance(past_key_values, PagedCache) and 0 in (past_key_values.planned or ()):
@@ -308,4 +310,7 @@ class LlamaForCausalLM(nn.Module):
                 done = token == eos_token_id
             tokens.append(token)
             input_ids = token.clamp(min=0)[:, None]          # -1 (nothing to draw) is no row of the embedding
-        return torch.stack(tokens, dim=1) if tokens else torch.empty((0, 0), dtype=torch.int64, device=input_ids.device)
+        if not tokens:
+            batch = past_key_values.batch if isinstance(past_key_values, PagedCache) else input_ids.shape[0]
+            return torch.empty((batch, 0), dtype=torch.int64, device=input_ids.device)
+        return torch.stack(tokens, dim=1)

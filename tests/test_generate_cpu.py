@@ -90,3 +90,14 @@ def test_generate_never_embeds_what_was_not_drawn(pkg, monkeypatch, eos):
         assert got.tolist() == [[3, 5, -1, 4], [-1, -1, 2, 4]] and r.seen[1:] == [[[3], [0]], [[5], [0]], [[0], [2]]]
     if eos == 5:
         assert got[0].tolist() == [3, 5, 5, 5]
+
+
+def test_generate_nothing(pkg):
+    """No token for each sequence, a packed prompt's too; the cache stays as it is."""
+    model, cache = small(pkg), paged(pkg)
+    cache.plan([4, 1, 3])
+    assert tuple(model.generate(torch.zeros(1, 8, dtype=torch.int64), cache, 0).shape) == (3, 0)
+    assert tuple(model.generate(torch.zeros(2, 8, dtype=torch.int64), None, 0).shape) == (2, 0)
+    assert cache.planned == [4, 1, 3] and cache.lengths == [0, 0, 0]
+    with pytest.raises(ValueError):
+        model.generate(torch.zeros(2, 8, dtype=torch.int64), None, -1)
