@@ -243,8 +243,12 @@ class LlamaModel(nn.Module):
         if isinstance(past_key_values, PagedCache):
             # positions follow from the cache's lengths, and rotation happens where the keys are stored
             past_key_values.begin_step(*input_ids.shape)
-            for layer in self.layers:
-                h = layer(h, past_key_value=past_key_values, position_ids=position_ids)
+            try:
+                for layer in self.layers:
+                    h = layer(h, past_key_value=past_key_values, position_ids=position_ids)
+            except Exception:
+                past_key_values.cancel_step()
+                raise
             return self.norm(h)
         if position_ids is None:
             past = past_key_values._seen_tokens if past_key_values is not None else 0

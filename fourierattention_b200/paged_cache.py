@@ -56,6 +56,7 @@ class PagedCache(Cache):
         self._free: List[int] = list(range(self.num_pages - 1, -1, -1))
         self._plan: Optional[List[int]] = None              # new tokens of the next step, where given
         self._prefix_ids: List[int] = []
+        self._before = None                                 # lengths and plan before the step begun last
 
     # -------------------------------------------------------------------------------------------- steps
     def plan(self, new_tokens: Sequence[int]):
@@ -86,6 +87,7 @@ class PagedCache(Cache):
         grow = [-(-n // self.page_size) - len(p) for n, p in zip(lengths, self._pages)]
         if sum(grow) > len(self._free):
             raise RuntimeError(f"PagedCache: {sum(grow)} pages wanted, {len(self._free)} of {self.num_pages} are free")
+        self._before = self.lengths, self._plan
         self._plan = None
         for b, n in enumerate(grow):
             for _ in range(n):
@@ -102,6 +104,15 @@ class PagedCache(Cache):
                 at.append(at[-1] + n)
             self.kv_lens.copy_(torch.tensor(lengths, dtype=torch.int32))
             self.cu_seqlens = torch.tensor(at, dtype=torch.int32, device=self.device)
+
+    def cancel_step(self):
+        """Takes back the step begun last, for one whose layers failed: the cache and its plan are as before."""
+        if self._before is None:
+            raise RuntimeError("cancel_step: no step has been begun")
+        lengths, self._plan = self._before
+        self._before = None
+        for b, n in enumerate(lengths):
+            self.truncate(b, n)
 
     def _upload_table(self):
         self.page_table.copy_(torch.tensor([p + [0] * (self.max_pages - len(p)) for p in self._pages], dtype=torch.int32))
@@ -136,6 +147,7 @@ class PagedCache(Cache):
             raise RuntimeError("share_prefix: the other sequences must be empty")
         if not self.lengths[sequence]:
             raise RuntimeError("share_prefix: the sequence is empty")
+        self._before = None
         self._prefix_ids, self.prefix_len = self._pages[sequence], self.lengths[sequence]
         self.prefix_pages = torch.tensor(self._prefix_ids, dtype=torch.int32, device=self.device)
         self._pages[sequence], self.lengths[sequence] = [], 0
@@ -146,6 +158,7 @@ class PagedCache(Cache):
         its place takes another)."""
         if not 0 <= length <= self.lengths[sequence]:
             raise ValueError(f"truncate: {length} of {self.lengths[sequence]} tokens")
+        self._before = None
         keep = -(-length // self.page_size)
         self._free.extend(reversed(self._pages[sequence][keep:]))
         self._pages[sequence] = self._pages[sequence][:keep]

@@ -101,3 +101,16 @@ def test_generate_nothing(pkg):
     assert cache.planned == [4, 1, 3] and cache.lengths == [0, 0, 0]
     with pytest.raises(ValueError):
         model.generate(torch.zeros(2, 8, dtype=torch.int64), None, -1)
+
+
+def test_a_failed_forward_leaves_the_cache(pkg):
+    """Here the cache's type is not the model's; the lengths must not count keys that were never stored."""
+    model, cache = small(pkg), paged(pkg)                        # float32 model, bfloat16 cache
+    for plan, shape in (([4, 1, 3], (1, 8)), (None, (3, 2))):
+        if plan:
+            cache.plan(plan)
+        with torch.no_grad(), pytest.raises((ValueError, RuntimeError)):
+            model(torch.zeros(shape, dtype=torch.int64), past_key_values=cache)
+        assert cache.lengths == [0, 0, 0] and cache.kv_lens.tolist() == [0, 0, 0] and cache.planned == plan
+        assert len(cache._free) == cache.num_pages
+        cache._plan = None

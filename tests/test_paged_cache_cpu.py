@@ -103,3 +103,27 @@ def test_last_rows_of_idle_sequences(PagedCache, new):
         at += n
         want = h[0, at - 1] if n else torch.zeros(2)
         assert torch.equal(got[b, 0].nan_to_num(-1.0), want.nan_to_num(-1.0))
+
+
+def test_a_cancelled_step_leaves_no_trace(PagedCache):
+    c = make(PagedCache)
+    with pytest.raises(RuntimeError, match="no step"):
+        c.cancel_step()
+    c.plan([17, 0, 16])
+    c.begin_step(1, 33)
+    pages, free = [list(p) for p in c._pages], sorted(c._free)
+    for plan in ([3, 20, 0], None):
+        if plan:
+            c.plan(plan)
+        c.begin_step(*((1, 23) if plan else (3, 1)))
+        c.cancel_step()
+        assert c.lengths == [17, 0, 16] and c.kv_lens.tolist() == [17, 0, 16] and c.planned == plan
+        assert c._pages == pages and sorted(c._free) == free
+        c._plan = None
+    with pytest.raises(RuntimeError, match="no step"):
+        c.cancel_step()
+    c.begin_step(3, 1)
+    assert c.kv_lens.tolist() == [18, 1, 17] and c.page_table[1, 0] == c._pages[1][0]
+    c.truncate(0, 4)                                # what was done since cannot be taken back with it
+    with pytest.raises(RuntimeError, match="no step"):
+        c.cancel_step()
