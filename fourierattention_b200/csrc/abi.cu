@@ -4,7 +4,7 @@
 #include <mutex>
 #include <string.h>
 
-#include "common.cuh"
+#include "serving.cuh"
 
 namespace fa {
 

@@ -8,8 +8,6 @@
 #include <stdint.h>
 #include <stdio.h>
 
-#include <atomic>
-
 #include "fourier_b200.h"
 
 namespace fa {
@@ -112,27 +110,10 @@ inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int sm_count();
 
-// Raises a kernel's limit of dynamic shared memory, once per device.
-template <auto Kernel>
-inline int allow_smem(int bytes, const char* what) {
-  static std::atomic<uint64_t> done{0};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && dev < 64 && ((done.load(std::memory_order_relaxed) >> dev) & 1)) return FA_OK;
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return cuda_fail(e, what);
-  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
-  return FA_OK;
-}
-
 // (cols x rows x B) tiled tensor map of a 16-bit tensor, 128-byte swizzle, out-of-range elements read as 0.
 // box_cols * 2 bytes must not exceed 128.  Strides in elements.
 int make_tensor_map_3d(CUtensorMap* m, const void* base, int dtype, int cols, int rows, int64_t row_stride, int B,
                        int64_t batch_stride, int box_cols, int box_rows);
-
-// (cols x rows x heads x pages) tiled tensor map of a 16-bit cache of pages, 128-byte swizzle; the same limits.
-int make_tensor_map_4d(CUtensorMap* m, const void* base, int dtype, int cols, int rows, int64_t row_stride, int heads,
-                       int64_t head_stride, int pages, int64_t page_stride, int box_cols, int box_rows);
 
 // tensor-core projection (compress_tc.cu)
 bool compress_tc_usable(const void* x, int B, int K, int64_t x_sb, int64_t x_sk, int x_cols, int N);

@@ -8,7 +8,7 @@
 // (unnormalised output, running maximum, denominator) in slots, two per CTA, that the merge kernel joins in order.
 #pragma once
 
-#include "common.cuh"
+#include "serving.cuh"
 
 namespace fa {
 

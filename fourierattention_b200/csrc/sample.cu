@@ -26,7 +26,7 @@
 // with the state behind a pointer it lived in local memory, and a row took 34 us.
 #include <cooperative_groups.h>
 
-#include "common.cuh"
+#include "serving.cuh"
 
 namespace cg = cooperative_groups;
 
