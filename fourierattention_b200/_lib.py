@@ -22,7 +22,7 @@ EXPORTS = ["fa_version", "fa_last_error_string", "fa_gather_cols", "fa_colstats"
            "fa_cache_step", "fa_evict_step", "fa_decode_scratch_bytes", "fa_decode_path", "fa_decode_attn", "fa_decode_attn_static", "fa_merge",
            "fa_layer_create", "fa_layer_destroy", "fa_layer_rebind_stores", "fa_layer_update", "fa_layer_scratch_bytes",
            "fa_layer_attend", "fa_layer_decode_path", "fa_qk_norm_rope", "fa_paged_append", "fa_paged_attn_scratch_bytes",
-           "fa_paged_attn", "fa_sample"]
+           "fa_paged_attn_launches", "fa_paged_attn", "fa_sample"]
 
 i32, i64, vp, f32, sz = C.c_int32, C.c_int64, C.c_void_p, C.c_float, C.c_size_t
 
@@ -158,6 +158,7 @@ def _load():
     lib.fa_paged_append.argtypes = [C.c_char_p, vp]
     lib.fa_paged_attn_scratch_bytes.argtypes = [C.c_char_p]
     lib.fa_paged_attn_scratch_bytes.restype = sz
+    lib.fa_paged_attn_launches.argtypes = [C.c_char_p]
     lib.fa_paged_attn.argtypes = [C.c_char_p, vp]
     lib.fa_sample.argtypes = [vp, C.c_int, C.c_int, C.c_int, i64, vp, vp, f32, vp, C.c_int, vp, f32, vp, f32, vp, vp, vp]
     for name in EXPORTS:

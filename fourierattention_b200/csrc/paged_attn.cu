@@ -647,6 +647,11 @@ extern "C" size_t fa_paged_attn_scratch_bytes(const fa_paged_attn_args_t* args_h
   return pa_plan(args_host).bytes;
 }
 
+extern "C" int fa_paged_attn_launches(const fa_paged_attn_args_t* a) {
+  if (pa_check(a) != FA_OK || a->tokens == 0 || a->B == 0) return 0;
+  return a->prefix_len > 0 && !pa_plan(a).lead ? 3 : 2;
+}
+
 extern "C" int fa_paged_attn(const fa_paged_attn_args_t* a, fa_stream_t stream) {
   const int rc = pa_check(a);
   if (rc != FA_OK) return rc;

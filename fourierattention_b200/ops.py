@@ -575,7 +575,7 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e
                        positions.data_ptr(), inv_freq.data_ptr(), qw, kw, eps, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
                        0, 0)
     _call(lib.fa_qk_norm_rope, "fa_qk_norm_rope", index, a)
-    _count(1)
+    _count(1 if tokens else 0)
     return q_out, k_out
 
 
@@ -645,7 +645,7 @@ def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, inv_freq, cu_seqle
                        vp[1], vp[2], page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(),
                        cu_seqlens.data_ptr() if cu_seqlens is not None else 0, pos_offset)
     _call(lib.fa_paged_append, "fa_paged_append", index, a)
-    _count(1)
+    _count(1 if tokens and B else 0)
     return q_out
 
 
@@ -695,7 +695,9 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens=None, p
             rc = _paged_attention(block, q, index)
     if rc:
         check(rc, "fa_paged_attn")
-    _count(3 if prefix_len else 2)
+    # (asked for only where it is not plain: a prefix under several new tokens)
+    _count(lib.fa_paged_attn_launches(bytes(block)) if prefix_len and cu_seqlens is not None
+           else (3 if prefix_len else 2) if tokens and B else 0)
     return (out, lse) if return_lse else out
 
 
@@ -747,7 +749,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_log
     logprob = u.new_empty((B,)) if return_logprob else None
     _call(lib.fa_sample, "fa_sample", index, logits.data_ptr(), code, B, V, stride[0], u.data_ptr(), tp, tv, kp, kv, pp, pv,
           mp, mv, token.data_ptr(), logprob.data_ptr() if return_logprob else None)
-    _count(1)
+    _count(1 if B else 0)
     return (token, logprob) if return_logprob else token
 
 

@@ -359,6 +359,7 @@ typedef struct {
  * token sees kv_lens[b] keys, each one before it a key less.  The prefix is read once for the whole batch.  A row
  * without keys gives 0, lse -infinity. */
 size_t fa_paged_attn_scratch_bytes(const fa_paged_attn_args_t* args_host);
+int fa_paged_attn_launches(const fa_paged_attn_args_t* args_host); /* kernels a call runs: 0 to 3 */
 int fa_paged_attn(const fa_paged_attn_args_t* args_host, fa_stream_t stream);
 
 /* One token per row of logits (B, V), V <= 393216.  Weights w_i = exp((x_i - max x) / temperature), in the order

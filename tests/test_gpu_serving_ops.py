@@ -705,3 +705,37 @@ def test_sample_odd_filter_values(ops, V, top_k):
         check_sample(ops, x, u, top_k=top_k, **kw)
     check_sample(ops, x, u, top_k=top_k, min_p=1.0)             # all nine
     assert torch.equal(ops.sample(x, u, temperature=full(nan)), ops.sample(x, u, temperature=0.0))
+
+
+def kernels_of(f):
+    """Number of kernels that ``f`` puts into a captured graph."""
+    rt = pytest.importorskip("cuda.bindings.runtime")
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g):
+        f()
+    raw = rt.cudaGraph_t(init_value=g.raw_cuda_graph())
+    n = rt.cudaGraphGetNodes(raw)[2]
+    nodes = rt.cudaGraphGetNodes(raw, n)[1] if n else []
+    return sum(rt.cudaGraphNodeGetType(x)[1] == rt.cudaGraphNodeType.cudaGraphNodeTypeKernel for x in nodes)
+
+
+@pytest.mark.parametrize("new,prefix", [(None, 0), (None, 40), (1, 40), (30, 40), (30, 0), (47, 40), (48, 40), (200, 40), (0, 40),
+                                        (0, 0)])
+def test_launches_are_counted_as_they_are(ops, new, prefix):
+    """Two kernels without a prefix, three with one, two again where it is read in front of the sequences' own keys; none
+    for an empty call."""
+    B, d, hkv, hq = 2, 64, 2, 8
+    kp, vp, table, pre = make_pages([256, 256], hkv, d, 16, BF)
+    kp.zero_(), vp.zero_()
+    t = B if new is None else B * new
+    q, kv = torch.zeros(t, hq, d, device="cuda", dtype=BF), torch.zeros(t, hkv, d, device="cuda", dtype=BF)
+    lens = torch.tensor([256, 250], dtype=torch.int32, device="cuda")
+    cu = None if new is None else torch.tensor([0, new, 2 * new], dtype=torch.int32, device="cuda")
+    f, x, u, pos = inv_freq(d), torch.zeros(t, 50, device="cuda"), torch.zeros(t, device="cuda"), torch.arange(t, device="cuda")
+    for call in (lambda: ops.paged_attention(q, kp, vp, table, lens, cu_seqlens=cu, prefix_pages=pre, prefix_len=prefix),
+                 lambda: ops.paged_append(kv, kv, kp, vp, table, lens, f, cu_seqlens=cu),
+                 lambda: ops.qk_norm_rope(q, kv, pos, f), lambda: ops.sample(x, u)):
+        call()
+        before = ops.launch_count
+        n = kernels_of(call)
+        assert ops.launch_count - before == n
