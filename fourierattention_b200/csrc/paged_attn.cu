@@ -12,10 +12,11 @@ namespace fa {
 // waits for another while keys stream.  The products are turned round, keys as the 16 rows of mma.m16n8k16 and query
 // rows as its 8 columns: a group of up to 8 query heads fills the instruction, where query rows as the 16 rows would
 // leave half of it empty and twice the accumulator registers.  The running maximum moves only when a score passes it
-// by 2^8 (one vote per 16 keys instead of three shuffle rounds); until then probabilities stay below 2^8, inside
-// fp16's range, and the denominator sums what was not rounded.  Measured: 6.1 TB/s (93 % of the copy rate) for 32 sequences
+// by 2^8 (one vote per 16 keys instead of three shuffle rounds); until then probabilities stay inside fp16's range (PaLift),
+// and the denominator sums what was not rounded.  Measured: 6.1 TB/s (93 % of the copy rate) for 32 sequences
 // of up to 16384 keys, 24 / 8 heads; ring of 24 KB per warp, 192 KB per SM in flight.  Probabilities are rounded to the cache's type for the
-// second product (relative error 2^-9 / 2^-12, independent from key to key).
+// second product (relative error up to 2^-9 in bf16 and, from 2^-21 of the largest up, 2^-12 in fp16; independent from key
+// to key).
 template <int D>
 struct PaStream {
   static constexpr int WARPS = 8;
@@ -80,6 +81,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
   float* obuf = reinterpret_cast<float*>(pa_dyn + C::RING);
   typename C::Small& sh = *reinterpret_cast<typename C::Small*>(pa_dyn + C::RING + C::OBUF);
   const uint32_t bar0 = pa_smem(&sh.bar[warp][0]);
+  constexpr float LIFT = PaLift<T>::STEPS;
 
   if (tid == 0) {
     sh.dead = 0;
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
             s[nt][j] *= c.scale_log2;
             if (masked && tok + g + 8 * (j >> 1) >= lim[nt][j & 1]) s[nt][j] = -INFINITY;
           }
-          rise |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + 8.f || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + 8.f;
+          rise |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + (8.f + LIFT) || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + (8.f + LIFT);
         }
         if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              mx = fmaxf(mx, m[nt][j]);
+              mx = fmaxf(mx - LIFT, m[nt][j]);
               const float f = m[nt][j] == -INFINITY ? 0.f : pa_ex2(m[nt][j] - mx);
               m[nt][j] = mx;
               l[nt][j] *= f;

@@ -253,6 +253,18 @@ __device__ __forceinline__ float pa_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
+// Probabilities are 2^(s - m) with m the running maximum less this many steps.  In fp16 a probability 2^-14 below the
+// largest would lose bits and one 2^-25 below it vanish, and many keys that far behind a dominant one (a first token that
+// draws the attention to itself) add up to what counts; seven steps higher, the largest still fit (2^15: the maximum may
+// lag by 2^8) and bits are lost from 2^-21 on.  bf16 has float32's range.
+template <typename T>
+struct PaLift {
+  static constexpr float STEPS = 0.f;
+};
+template <>
+struct PaLift<__half> {
+  static constexpr float STEPS = 7.f;
+};
 template <typename T>
 __device__ __forceinline__ uint32_t pa_pack(float lo, float hi);
 template <>

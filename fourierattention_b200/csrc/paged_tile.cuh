@@ -19,7 +19,7 @@
 //   warp 19          completes the warpgroup that gives its registers away
 // Tensor memory (512 columns): S0, S1 (128 each; P overwrites the first half of its S), O0, O1.  MMAs execute in the order
 // of their issue, so S of the next tile may be issued behind the product that still reads P.  The running maximum moves
-// only when a row passes it by 2^8; then the row's thread rescales its accumulator in tensor memory, which nothing else
+// only when a row passes it by 2^8 (more in fp16: PaLift); then the row's thread rescales its accumulator in tensor memory, which nothing else
 // touches at that point: the product before has completed (the commit that announced S covers it), the next one waits
 // for P.  The second half of a row writes its P over scores of the first half, behind the vote, when those are read.
 #pragma once
@@ -217,6 +217,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     const uint32_t ts = tmem + w * 128 + lanes, to = tmem + 256 + w * 128 + lanes;
     const uint32_t s_full = pa_smem(&sh.s_full[w]), p_full = pa_smem(&sh.p_full[w]);
     const float scale = c.scale_log2;
+    constexpr float LIFT = PaLift<T>::STEPS;
     uint32_t s_par = 0, o_par = 0;
     int tile_no = 0;                                      // tiles since the start
     for (int seg_no = 0;; ++seg_no) {
@@ -281,10 +282,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
 #pragma unroll
             for (int k = 0; k < 4; ++k) mx[k] = pt_max3(mx[k], __uint_as_float(sr[j + k]), __uint_as_float(sr[j + 4 + k]));
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-          if (pt_sync_any(1 + w, top > m + 8.f)) {
+          if (pt_sync_any(1 + w, top > m + (8.f + LIFT))) {
             sh.half[w][half][i] = top;
             pt_sync(1 + w);
-            const float nm = fmaxf(m, fmaxf(top, sh.half[w][half ^ 1][i]));
+            const float nm = fmaxf(m, fmaxf(top, sh.half[w][half ^ 1][i]) - LIFT);
             const float f = m == -INFINITY ? 0.f : pa_ex2(m - nm);
             m = nm;
             l *= f;

@@ -739,3 +739,41 @@ def test_launches_are_counted_as_they_are(ops, new, prefix):
         before = ops.launch_count
         n = kernels_of(call)
         assert ops.launch_count - before == n
+
+
+@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("dtype", [HF, BF])
+@pytest.mark.parametrize("shared", [False, True])
+def test_attention_many_small_probabilities(ops, new, dtype, shared):
+    """Keys far behind a few dominant ones, whose values are zero, make up the output: each of their probabilities has to
+    keep its bits.  They are 2^-20.6 of the largest; below 2^-21 of it a float16 probability is off by up to 2^-32 of the
+    largest, so n keys add n 2^-32 max |v| / (weight of the dominant ones) to the tolerance."""
+    d, ps, hkv, n, B = 64, 64, 8, 20000, 20
+    kp, vp, table, _ = make_pages([n], hkv, d, ps, dtype)
+    k, v = torch.zeros(n, hkv, d, device="cuda"), torch.rand(n, hkv, d, device="cuda") + 0.5
+    far, near = -14.25, torch.arange(0, 128, 16, device="cuda")
+    k[:, :, 0] = far
+    k[near] = 0.0
+    v[near] = 0.0
+    k, v = k.to(dtype), v.to(dtype)
+    for j0 in range(0, n, ps):
+        m = min(ps, n - j0)
+        kp[int(table[0, j0 // ps]), :, :m], vp[int(table[0, j0 // ps]), :, :m] = k[j0:j0 + m].transpose(0, 1), v[j0:j0 + m].transpose(0, 1)
+    q = torch.zeros(B * new, hkv, d, device="cuda", dtype=dtype)
+    q[:, :, 0] = 1.0
+    cu = None if new == 1 else torch.arange(0, B * new + 1, new, dtype=torch.int32, device="cuda")
+    if shared:
+        out, lse = ops.paged_attention(q, kp, vp, torch.zeros((B, 1), dtype=torch.int32, device="cuda"),
+                                       torch.zeros(B, dtype=torch.int32, device="cuda"), cu_seqlens=cu, prefix_pages=table[0],
+                                       prefix_len=n, sm_scale=1.0, return_lse=True)
+        own, args = 0, (k, v)
+    else:
+        out, lse = ops.paged_attention(q, kp, vp, table.expand(B, -1), torch.full((B,), n, dtype=torch.int32, device="cuda"),
+                                       cu_seqlens=cu, sm_scale=1.0, return_lse=True)
+        own, args = n, (k[:0], v[:0])
+    one = (k[:own], v[:own])
+    o, rl, a, e = attend_ref(q[:new], [new], [own], [one[0]], [one[1]], *args, 1.0)
+    h = half_step(dtype)
+    tol = h * o.abs() + (h + 2 * e + 2.0 ** -18) * a + n * 2.0 ** -32 * 1.5 / 8 + 2.0 ** -24
+    assert excess((out.double().view(B, new, hkv, d) - o).abs(), tol.expand(B, new, hkv, d)) <= 0
+    assert excess((lse.double().view(B, new, hkv) - rl[..., 0]).abs(), (e[..., 0] + 2.0 ** -18 + 2.0 ** -22 * rl[..., 0].abs()).expand(B, new, hkv)) <= 0
