@@ -777,3 +777,63 @@ def test_attention_many_small_probabilities(ops, new, dtype, shared):
     tol = h * o.abs() + (h + 2 * e + 2.0 ** -18) * a + n * 2.0 ** -32 * 1.5 / 8 + 2.0 ** -24
     assert excess((out.double().view(B, new, hkv, d) - o).abs(), tol.expand(B, new, hkv, d)) <= 0
     assert excess((lse.double().view(B, new, hkv) - rl[..., 0]).abs(), (e[..., 0] + 2.0 ** -18 + 2.0 ** -22 * rl[..., 0].abs()).expand(B, new, hkv)) <= 0
+
+
+@pytest.mark.parametrize("ps", [16, 64, 256])
+@pytest.mark.parametrize("new", [1, 3, 30, 60])
+@pytest.mark.parametrize("where", ["own", "prefix", "both", "all"])
+def test_page_ids_that_name_no_page_in_every_form(ops, ps, new, where):
+    """Their keys do not exist, for both kernels, in the own pages and in a prefix (read for the batch or in front of the own
+    keys), with pages smaller and larger than a tile.  The pages that the ids used to name hold NaN."""
+    torch.manual_seed(ps + new)
+    d, hkv, hq, B, dtype = 128, 2, 8, 2, BF
+    own, prefix = [5 * ps + 3 + new, 2 * ps + new], 4 * ps - 5
+    kp, vp, table, _ = make_pages(own + [prefix], hkv, d, ps, dtype)
+    drop = {0: [0, 2], 1: [1], 2: [1, 3]}                       # pages of the two sequences and of the prefix
+    if where == "all":
+        drop = {i: list(range(table.shape[1])) for i in range(3)}
+    elif where != "both":
+        drop = {i: (p if (i == 2) == (where == "prefix") else []) for i, p in drop.items()}
+    keys, values = [], []
+    for i, n in enumerate(own + [prefix]):
+        k, v = torch.randn(n, hkv, d, device="cuda").to(dtype), torch.randn(n, hkv, d, device="cuda").to(dtype)
+        for j in range(-(-n // ps)):
+            m = min(ps, n - j * ps)
+            if j in drop[i]:
+                table[i, j] = -1 - j if j % 2 else kp.shape[0] + 7 * j
+            else:
+                kp[int(table[i, j]), :, :m] = k[j * ps:j * ps + m].transpose(0, 1)
+                vp[int(table[i, j]), :, :m] = v[j * ps:j * ps + m].transpose(0, 1)
+        keys.append(k)
+        values.append(v)
+    q = (2 * torch.randn(B * new, hq, d, device="cuda")).to(dtype)
+    cu = torch.arange(0, B * new + 1, new, dtype=torch.int32, device="cuda")
+    out, lse = ops.paged_attention(q, kp, vp, table[:2], torch.tensor(own, dtype=torch.int32, device="cuda"), cu_seqlens=cu,
+                                   prefix_pages=table[2, :4].contiguous(), prefix_len=prefix, return_lse=True)
+    there = lambda i, n: torch.tensor([j // ps not in drop[i] for j in range(n)], device="cuda")
+    pre_there = there(2, prefix)
+    for b in range(B):
+        for i in range(new):                                    # a token at a time: what it sees, less what is not there
+            sees = own[b] - new + 1 + i
+            keep = there(b, own[b])[:sees]
+            k, v = torch.cat([keys[2][pre_there], keys[b][:sees][keep]]), torch.cat([values[2][pre_there], values[b][:sees][keep]])
+            o, rl, a, e = attend_ref(q[b * new + i][None], [1], [len(k)], [k], [v], k[:0], v[:0], d ** -0.5)
+            h, got = half_step(dtype), out[b * new + i]
+            if not len(k):
+                assert bool((got == 0).all()) and bool((lse[b * new + i] == -math.inf).all())
+                continue
+            assert excess((got.double() - o[0]).abs(), (h * o.abs() + (h + 2 * e + 2.0 ** -18) * a + 2.0 ** -24)[0]) <= 0
+            assert excess((lse[b * new + i].double() - rl[0, :, 0]).abs(), e[0, :, 0] + 2.0 ** -18 + 2.0 ** -22 * rl[0, :, 0].abs()) <= 0
+
+
+@pytest.mark.parametrize("V", [131073, 151936, 262145, 393215])
+def test_sample_long_rows_of_any_alignment(ops, V):
+    """Several rounds per CTA; rows that start off 16 bytes, with and without room for what leads them in."""
+    torch.manual_seed(V)
+    for dtype in (torch.float32, HF):
+        x, u = (3 * torch.randn(3, V, device="cuda")).to(dtype), torch.rand(3, device="cuda")
+        check_sample(ops, x, u)
+        check_sample(ops, x, u, top_k=50, top_p=0.9)
+        check_sample(ops, x, u, top_k=3000, min_p=1e-4)
+        check_sample(ops, x, u, top_p=0.95, temperature=0.8)
+        check_sample(ops, x, u, temperature=0.0)
