@@ -26,6 +26,7 @@
 // with the state behind a pointer it lived in local memory, and a row took 34 us.
 #include <cooperative_groups.h>
 
+#include "sample_exp.cuh"
 #include "serving.cuh"
 
 namespace cg = cooperative_groups;
@@ -61,7 +62,7 @@ struct SaXchg {
 };
 
 struct SaShared {
-  double exp2[64];            // 2^(i / 64)
+  double exp2[SA_EXP_TABLE];
   uint32_t hist[SA_BINS];
   SaXchg x[2];
   float lx[SA_LIST];          // this CTA's part of a bin
@@ -78,24 +79,6 @@ struct SaShared {
 };
 
 __device__ __forceinline__ double shfl_up_d(double v, int o) { return __shfl_up_sync(0xffffffffu, v, o); }
-// e^z for z <= 0, to a few units of 2^-53: z = (n / 64) ln 2 + r with |r| <= ln 2 / 128 and n rounded by adding
-// 1.5 * 2^52; 2^((n mod 64) / 64) from a table, the Taylor polynomial of degree 5 (remainder r^6 / 720 = 4e-17), n / 64
-// added to the exponent.  Below e^-700: 0.
-__device__ __forceinline__ double sa_exp(double z, const double* table) {
-  const double t = fma(z, 64.0 * 1.4426950408889634, 6755399441055744.0);
-  const int n = __double2loint(t);
-  const double nf = t - 6755399441055744.0;
-  double r = fma(nf, -0.6931471805599453 / 64.0, z);  // ln 2 as a sum of two doubles
-  r = fma(nf, -2.3190468138462996e-17 / 64.0, r);
-  double p = 1.0 / 120.0;
-  p = fma(p, r, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0) * table[n & 63];
-  const double e = __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p));
-  return z < -700.0 ? 0.0 : e;
-}
 // The bin of a distance from the largest logit: the nearest multiple of 1 / scale, by adding 2^23 (a conversion to an
 // integer takes the slow pipe, which the exponentials need).  Monotone in d; 0 for d = 0 even where scale is infinite.
 __device__ __forceinline__ int sa_bin(float d, float scale) {
@@ -636,7 +619,7 @@ struct Sampler {
     if (!vec) lead = 0;
     base = rank * p.slice - lead;
     n = max(0, min(p.V - base, p.slice));
-    if (tid < 64) sh.exp2[tid] = exp2((double)tid / 64.0);
+    if (tid < SA_EXP_TABLE) sh.exp2[tid] = exp2((double)tid / SA_EXP_TABLE);
     const float temperature = p.temperature ? p.temperature[row] : p.temperature0;
     // a NaN filter is off; min_p above 1 leaves the largest logit alone, as top_k = 1 does
     float top_p = p.top_p ? p.top_p[row] : p.top_p0;
