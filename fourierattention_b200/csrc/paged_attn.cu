@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
     }
     const int t_end = (int)min((long long)u.tiles, t + (range.end - done));
     // ---- the block's query rows, as the second operand -------------------------------------------------------------
-    const int row0 = u.rb << p.rows_log2;
+    const int row0 = u.rb << p.rows_log2, L = pa_keys(p, u.s);
     const int n_rows = min(1 << p.rows_log2, u.s.n * c.G - row0);
     uint32_t qf[NT][D / 16][2];
     int lim[NT][2];
@@ -179,10 +179,10 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int rr = min(nt * 8 + c2 + j, n_rows - 1);
-        lim[nt][j] = p.prefix_len > 0 ? u.s.L : min(u.s.L, u.s.len - u.s.n + (row0 + rr) / c.G + 1);
+        lim[nt][j] = p.prefix_len > 0 ? L : min(L, u.s.len - u.s.n + (row0 + rr) / c.G + 1);
       }
     }
-    const int lim0 = p.prefix_len > 0 ? u.s.L : min(u.s.L, u.s.len - u.s.n + row0 / c.G + 1);     // the first row sees least
+    const int lim0 = p.prefix_len > 0 ? L : min(L, u.s.len - u.s.n + row0 / c.G + 1);     // the first row sees least
     float o[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -248,11 +248,11 @@ __global__ void __launch_bounds__(256, 1) paged_stream_kernel(const __grid_const
           pb[nt][0] = pa_turn(pa_pack<T>(p0, p1));
           pb[nt][1] = pa_turn(pa_pack<T>(p2, p3));
         }
-        if (tok + 16 > u.s.L) {
+        if (tok + 16 > L) {
           // rows behind the sequence hold anything: 0 x NaN must not reach the sums
           for (int i = lane; i < 16 * (D / 8); i += 32) {
             const int r = i / (D / 8), ch = i % (D / 8);
-            if (tok + r >= u.s.L)
+            if (tok + r >= L)
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(vb + (ch >> 3) * C::BOX + r * 128 + ((ch & 7) << 4)), "r"(0) : "memory");
           }
           asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // before the next fetch into this stage
@@ -608,7 +608,8 @@ static int pa_run(const fa_paged_attn_args_t* a, cudaStream_t st) {
     PaPhase p;
     p.table = i == 0 ? a->page_table : a->prefix_pages;
     p.table_sb = i == 0 ? a->table_sb : 0;
-    p.max_pages = i == 0 ? a->max_pages : a->n_prefix_pages;
+    // (checked to be below 2^31; a prefix has its pages)
+    p.cap = i == 0 ? (int)((int64_t)a->max_pages * a->page_size) : a->prefix_len;
     p.prefix_len = i == 0 ? 0 : a->prefix_len;
     p.lead_table = a->prefix_pages;
     p.lead_len = i == 0 && pl.lead ? a->prefix_len : 0;

@@ -17,7 +17,7 @@ constexpr int PA_TILE = 128;
 struct PaPhase {
   const int32_t* table;      // (B, max_pages), or the prefix's pages
   int64_t table_sb;
-  int max_pages;
+  int cap;                   // keys that the table has room for
   int prefix_len;            // > 0: the shared prefix, every row sees all of it; 0: each sequence's own pages, causal
   const int32_t* lead_table; // own pages only: the pages of `lead_len` keys that come before them (tile kernel)
   int lead_len;
@@ -44,7 +44,7 @@ struct PaCommon {
 };
 
 struct PaSeq {
-  int t0, n, L, len;         // first new token, number of new tokens, number of keys that have a page, length
+  int t0, n, len;            // first new token, number of new tokens, length (which the table may not hold)
 };
 
 __device__ __forceinline__ PaSeq pa_seq(const PaCommon& c, const PaPhase& p, int b) {
@@ -52,27 +52,27 @@ __device__ __forceinline__ PaSeq pa_seq(const PaCommon& c, const PaPhase& p, int
   if (p.prefix_len > 0) {
     s.t0 = 0;
     s.n = c.cu ? max(0, min(c.tokens, c.cu[c.B])) : c.tokens;
-    s.L = s.len = p.prefix_len;
+    s.len = p.prefix_len;
     return s;
   }
   int t0 = b, t1 = b + 1;
   if (c.cu) t0 = c.cu[b], t1 = c.cu[b + 1];
   s.t0 = max(0, min(t0, c.tokens));
   s.n = max(0, min(t1, c.tokens) - s.t0);
-  // a token's place counts from the length as it is; keys behind the table do not exist
   s.len = max(0, c.kv_lens[b]);
-  s.L = (int)min((long long)s.len, (long long)p.max_pages * c.page_size);
   return s;
 }
+// keys that exist: those behind the table do not, but a token's place counts from the length as it is
+__device__ __forceinline__ int pa_keys(const PaPhase& p, const PaSeq& s) { return min(s.len, p.cap); }
 __device__ __forceinline__ int pa_seqs(const PaCommon& c, const PaPhase& p) { return p.prefix_len > 0 ? 1 : c.B; }
 __device__ __forceinline__ int pa_blocks(const PaCommon& c, const PaPhase& p, const PaSeq& s) {
   return (s.n * c.G + (1 << p.rows_log2) - 1) >> p.rows_log2;      // (tokens x G and a block more fit into 31 bits)
 }
 // keys seen by the last row of a block (a later token sees more)
 __device__ __forceinline__ int pa_limit(const PaCommon& c, const PaPhase& p, const PaSeq& s, int rb) {
-  if (p.prefix_len > 0) return s.L;
+  if (p.prefix_len > 0) return s.len;
   const int last = min(s.n * c.G, (rb + 1) << p.rows_log2) - 1;
-  return max(0, min(s.L, s.len - s.n + (int)((unsigned)last / (unsigned)c.G) + 1));
+  return max(0, min(pa_keys(p, s), s.len - s.n + (int)((unsigned)last / (unsigned)c.G) + 1));
 }
 __device__ __forceinline__ int pa_tiles(int limit) { return (limit + PA_TILE - 1) / PA_TILE; }
 // tiles of a unit whose rows see `limit` keys; those of the lead come first, in tiles of their own
@@ -80,7 +80,7 @@ __device__ __forceinline__ int pa_unit_tiles(const PaPhase& p, int limit) { retu
 __device__ __forceinline__ long long pa_head_tiles(const PaCommon& c, const PaPhase& p, const PaSeq& s) {
   const int nb = pa_blocks(c, p, s);
   if (nb == 0) return 0;
-  if (p.prefix_len > 0) return (long long)nb * pa_tiles(s.L);
+  if (p.prefix_len > 0) return (long long)nb * pa_tiles(s.len);
   long long sum = 0;
   for (int rb = 0; rb < nb; ++rb) sum += pa_unit_tiles(p, pa_limit(c, p, s, rb));
   return sum;

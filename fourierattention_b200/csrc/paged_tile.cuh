@@ -35,7 +35,7 @@ constexpr int PT_ROWS = 256;                              // rows_log2 = 8
 // a stretch of one unit's tiles, as the softmax warps need it; written ahead by a warp of its own, so that the walk and
 // its loads are off their path and take none of their registers
 struct PtSegment {
-  int more, row0, t0, n, L, len, h, t, t_end, first, last;   // more = 0: done
+  int more, row0, t0, n, len, h, t, t_end, first, last;   // more = 0: done
 };
 constexpr int PT_SEGS = 4;
 
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         __syncwarp();
         if (lane == 0) pa_bar_arrive(pa_smem(&sh.q_full[w]));
 
-        const int lim = p.prefix_len > 0 ? seg.L : min(seg.L, seg.len - seg.n + (row0 + min(i, n_rows - 1)) / c.G + 1);
+        const int lim = p.prefix_len > 0 ? seg.len : min(min(seg.len, p.cap), seg.len - seg.n + (row0 + min(i, n_rows - 1)) / c.G + 1);
         // keys of this half of the tile that the row sees, counted from the lead's or the sequence's first key
         const int lead = pa_tiles(p.lead_len);
         int tt = t_beg;
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     while (done < range.end) {
       const int key0 = (t < lead ? t : t - lead) * PA_TILE, nv = min(PA_TILE, (t < lead ? p.lead_len : u.limit) - key0);
       const int need = (nv + box_keys - 1) / box_keys;                // boxes with keys
-      const int row = (key0 + lane * box_keys) % c.page_size, head = u.h, L = t < lead ? p.lead_len : u.s.L;
+      const int row = (key0 + lane * box_keys) % c.page_size, head = u.h, L = t < lead ? p.lead_len : pa_keys(p, u.s);
       int page = next_id;
       const bool ok = lane >= need || (page >= 0 && page < c.num_pages);
       if (!ok) page = c.num_pages;                        // out of the map's range: zeros arrive
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         seg.t = t;
         seg.t_end = (int)min((long long)u.tiles, t + (range.end - done));
         seg.row0 = u.rb * PT_ROWS;
-        seg.t0 = u.s.t0, seg.n = u.s.n, seg.L = u.s.L, seg.len = u.s.len, seg.h = u.h;
+        seg.t0 = u.s.t0, seg.n = u.s.n, seg.len = u.s.len, seg.h = u.h;
         seg.first = seg.t == 0, seg.last = seg.t_end == u.tiles;
       }
       sh.seg[x] = seg;
