@@ -42,6 +42,8 @@ constexpr int SA_MAX_CLUSTER = 8;
 constexpr int SA_BINS = 1024;
 constexpr int SA_LIST = 512;
 constexpr int SA_MAX_VOCAB = SA_MAX_CLUSTER * SA_MAX_ROUNDS * SA_ROUND;
+constexpr int SA_STEPS = 8192;                     // of the largest weight in a bin; a bin of all elements fits 32 bits
+static_assert((unsigned long long)SA_MAX_VOCAB * SA_STEPS < 1ull << 32, "the bins of a histogram");
 
 struct SampleParams {
   const void* logits;
@@ -218,9 +220,8 @@ struct Sampler {
     out.n[0] = __shfl_sync(0xffffffffu, out.n[0], 0), out.n[1] = __shfl_sync(0xffffffffu, out.n[1], 0);
     xb ^= 1;
   }
-  // this thread's two bins of the histogram, over the cluster: a CTA's count of up to 49152 x 2^14 fits 32 bits, the sum
-  // of eight does not
-  __device__ __forceinline__ void read_bins(unsigned long long& a, unsigned long long& b) {
+  // this thread's two bins of the histogram, over the cluster (in 32 bits: SA_STEPS)
+  __device__ __forceinline__ void read_bins(unsigned& a, unsigned& b) {
     uint2 h[SA_MAX_CLUSTER];
 #pragma unroll
     for (int r = 0; r < SA_MAX_CLUSTER; ++r) {
@@ -344,13 +345,13 @@ struct Sampler {
       each([&](float x, int i) {
         if (!kept(x, i) || x > hi || x < lo) return;
         const int b = bin_of(x);
-        // weights relative to the bin's near edge, in steps of 2^-14
+        // weights relative to the bin's near edge, in steps of 1 / SA_STEPS
         const float rel = fminf(0.f, (x - hi + fmaxf(0.f, (float)b - 0.5f) * width) * c_w);
-        atomicAdd(&sh.hist[b], by_weight ? max(1u, __float_as_uint(fmaf(16384.f, __expf(rel), 8388608.f)) - 0x4b000000u) : 1u);
+        atomicAdd(&sh.hist[b], by_weight ? max(1u, __float_as_uint(fmaf((float)SA_STEPS, __expf(rel), 8388608.f)) - 0x4b000000u) : 1u);
       });
       cl.sync();
       // two neighbouring bins per thread, over the cluster
-      unsigned long long h0, h1;
+      unsigned h0, h1;
       read_bins(h0, h1);
       double v0 = (double)h0, v1 = (double)h1;
       if (by_weight) {
@@ -359,8 +360,8 @@ struct Sampler {
         v1 *= sa_exp((double)(((float)(2 * tid) + 0.5f) * width) * -inv_t, sh.exp2);
       }
       double total, pre = block_scan(v0 + v1, total) - (v0 + v1);   // what lies before this thread's bins
-      // the histogram counts weights in units of 2^-14 of the weight at hi
-      const double unit = by_weight ? 16384.0 / weight(hi) : 1.0;
+      // the histogram counts weights in units of 1 / SA_STEPS of the weight at hi
+      const double unit = by_weight ? (double)SA_STEPS / weight(hi) : 1.0;
       double target = by_weight ? fmin((goal - near) * unit, total) : (double)k - near;
 
       // ---- the bin's elements, and what lies before it --------------------------------------------------------
@@ -539,7 +540,7 @@ struct Sampler {
     __syncthreads();
     if (mine > -INFINITY) atomicAdd(&sh.hist[bin_of(mine)], 1u);
     cl.sync();
-    unsigned long long h0, h1;
+    unsigned h0, h1;
     read_bins(h0, h1);
     const int v0 = (int)h0, v1 = (int)h1;
     int pre = v0 + v1;
