@@ -49,6 +49,7 @@ class PagedCache(Cache):
         self.page_table = torch.zeros((batch, self.max_pages), dtype=torch.int32, device=self.device)
         self.kv_lens = torch.zeros((batch,), dtype=torch.int32, device=self.device)
         self.cu_seqlens: Optional[torch.Tensor] = None      # of the current step; None: one token per sequence
+        self._cu_seqlens = torch.zeros((batch + 1,), dtype=torch.int32, device=self.device)   # in one place: captured steps read it
         self.prefix_pages: Optional[torch.Tensor] = None
         self.prefix_len = 0
         self.lengths: List[int] = [0] * batch               # host copy of kv_lens
@@ -103,7 +104,8 @@ class PagedCache(Cache):
             for n in new:
                 at.append(at[-1] + n)
             self.kv_lens.copy_(torch.tensor(lengths, dtype=torch.int32))
-            self.cu_seqlens = torch.tensor(at, dtype=torch.int32, device=self.device)
+            self._cu_seqlens.copy_(torch.tensor(at, dtype=torch.int32))
+            self.cu_seqlens = self._cu_seqlens
 
     def cancel_step(self):
         """Takes back the step begun last, for one whose layers failed: the cache and its plan are as before."""

@@ -238,3 +238,50 @@ def test_qk_norm_in_front_of_the_fourier_cache():
         assert tuple(step.shape) == (B, 1, 211) and bool(torch.isfinite(step).all())
     with pytest.raises(RuntimeError, match="backward"):
         model(ids)
+
+
+def test_paged_steps_of_several_tokens_in_a_graph():
+    """A step of four tokens per sequence, then of four packed ones in changing shares, captured once and replayed while
+    lengths, pages and shares move on."""
+    from fourierattention_b200 import PagedCache
+    model = small_model(True)
+    draw = lambda n: torch.randint(211, (n,), generator=g).tolist()
+    for packed in (False, True):
+        g = torch.Generator().manual_seed(3)
+        cache = PagedCache(2, 2, 64, 2, 64, page_size=16, dtype=torch.float16)
+        seqs = [draw(9), draw(9)]
+        tok = torch.zeros((1, 8) if packed else (2, 4), dtype=torch.int64, device="cuda")
+
+        def step():
+            h = model.model.embed_tokens(tok)
+            for layer in model.model.layers:
+                h = layer(h, past_key_value=cache)
+            return model.lm_head(model.model.norm(h))
+        with torch.no_grad():
+            model(torch.tensor(seqs, device="cuda"), past_key_values=cache)
+            graph = None
+            for shares in ([4, 4], [3, 5], [7, 1], [2, 6], [0, 8]):
+                shares = shares if packed else [4, 4]
+                new = [draw(n) for n in shares]
+                if packed:
+                    cache.plan(shares)
+                cache.begin_step(*tok.shape)
+                tok.copy_(torch.tensor(sum(new, [])).view(tok.shape))
+                other = torch.full((64,), -1, dtype=torch.int32, device="cuda")      # takes memory that a step let go of
+                seqs = [s + n for s, n in zip(seqs, new)]
+                if graph is None:
+                    side = torch.cuda.Stream()
+                    side.wait_stream(torch.cuda.current_stream())
+                    with torch.cuda.stream(side):
+                        step()
+                    torch.cuda.current_stream().wait_stream(side)
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph):
+                        out = step()
+                graph.replay()
+                at = 0
+                for s, n in zip(seqs, shares):
+                    at += n
+                    if n:
+                        check_last(out.view(1, 8, -1)[:, :at], model, [s])
+                del other

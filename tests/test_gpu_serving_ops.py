@@ -837,3 +837,13 @@ def test_sample_long_rows_of_any_alignment(ops, V):
         check_sample(ops, x, u, top_k=3000, min_p=1e-4)
         check_sample(ops, x, u, top_p=0.95, temperature=0.8)
         check_sample(ops, x, u, temperature=0.0)
+
+
+@pytest.mark.parametrize("ps", [48, 80, 128, 1024])
+@pytest.mark.parametrize("layout", ["heads", "rows", "pairs"])
+def test_attention_pages_of_many_tokens(ops, ps, layout):
+    """Page sizes and layouts under the tensor-core kernel: a prefix as a phase of its own, and in front of the own keys."""
+    for new in ([70, 30], [20, 9, 30]):
+        own = [n + 333 * i for i, n in enumerate(new)]
+        for prefix in (0, 700):
+            check_attention(ops, new, own, prefix, 8, 2, 128, ps, HF, layout=layout, seed=ps, q_layout="wide", pad=1)

@@ -127,3 +127,19 @@ def test_a_cancelled_step_leaves_no_trace(PagedCache):
     c.truncate(0, 4)                                # what was done since cannot be taken back with it
     with pytest.raises(RuntimeError, match="no step"):
         c.cancel_step()
+
+
+def test_what_a_captured_step_reads_stays_in_place(PagedCache):
+    """Lengths, table and token offsets of a later step are where those of an earlier one were."""
+    c = make(PagedCache)
+    c.begin_step(3, 2)
+    where = lambda: (c.kv_lens.data_ptr(), c.page_table.data_ptr(), c.cu_seqlens.data_ptr())
+    first, held = where(), c.cu_seqlens
+    c.begin_step(3, 1)
+    assert c.cu_seqlens is None
+    c.plan([4, 0, 2])
+    c.begin_step(1, 6)
+    assert where() == first and held.tolist() == [0, 4, 4, 6]
+    c.reset()
+    c.begin_step(3, 3)
+    assert where() == first and held.tolist() == [0, 3, 6, 9]
