@@ -279,6 +279,9 @@ class LlamaForCausalLM(nn.Module):
             if packed and not (num_logits_to_keep in (0, 1) or num_logits_to_keep >= input_ids.shape[1]):
                 raise ValueError(f"num_logits_to_keep={num_logits_to_keep} of packed tokens: the rows would be of the last "
                                  "sequences only; 1 gives every sequence's last token, 0 all rows")
+            mask = kwargs.get("attention_mask")
+            if mask is not None and not bool((mask != 0).all()):
+                raise ValueError("a PagedCache takes sequences of different lengths packed (plan), not padded behind a mask")
         h = self.model(input_ids, past_key_values=past_key_values)
         if isinstance(past_key_values, PagedCache) and num_logits_to_keep == 1:
             h = past_key_values.last_rows(h)                 # of every sequence, packed or not

@@ -114,3 +114,15 @@ def test_a_failed_forward_leaves_the_cache(pkg):
         assert cache.lengths == [0, 0, 0] and cache.kv_lens.tolist() == [0, 0, 0] and cache.planned == plan
         assert len(cache._free) == cache.num_pages
         cache._plan = None
+
+
+def test_padded_batches_are_refused(pkg, monkeypatch):
+    """Padding would be stored and attended like tokens; a mask that hides nothing is taken."""
+    model, cache, ids = small(pkg), paged(pkg), torch.zeros(3, 4, dtype=torch.int64)
+    mask = torch.ones(3, 4, dtype=torch.int64)
+    mask[1, :2] = 0
+    with pytest.raises(ValueError, match="padded"):
+        model(ids, past_key_values=cache, attention_mask=mask)
+    assert cache.lengths == [0, 0, 0]
+    monkeypatch.setattr(model.model, "forward", lambda ids, past_key_values: past_key_values.begin_step(*ids.shape) or torch.zeros(3, 4, 64))
+    assert model(ids, past_key_values=cache, attention_mask=torch.ones_like(mask)).logits.shape == (3, 1, 11)
