@@ -282,7 +282,10 @@ class LlamaForCausalLM(nn.Module):
             mask = kwargs.get("attention_mask")
             if mask is not None and not bool((mask != 0).all()):
                 raise ValueError("a PagedCache takes sequences of different lengths packed (plan), not padded behind a mask")
-        h = self.model(input_ids, past_key_values=past_key_values)
+        positions = {}
+        if isinstance(past_key_values, PagedCache) and kwargs.get("position_ids") is not None:
+            positions = dict(position_ids=kwargs["position_ids"])
+        h = self.model(input_ids, past_key_values=past_key_values, **positions)
         if isinstance(past_key_values, PagedCache) and num_logits_to_keep == 1:
             h = past_key_values.last_rows(h)                 # of every sequence, packed or not
         logits = self.lm_head(h[:, -num_logits_to_keep:, :])

@@ -126,3 +126,17 @@ def test_padded_batches_are_refused(pkg, monkeypatch):
     assert cache.lengths == [0, 0, 0]
     monkeypatch.setattr(model.model, "forward", lambda ids, past_key_values: past_key_values.begin_step(*ids.shape) or torch.zeros(3, 4, 64))
     assert model(ids, past_key_values=cache, attention_mask=torch.ones_like(mask)).logits.shape == (3, 1, 11)
+
+
+def test_given_positions_reach_the_layers(pkg, monkeypatch):
+    model, cache, seen = small(pkg), paged(pkg), []
+
+    def layers(ids, past_key_values, position_ids=None):
+        seen.append(position_ids)
+        past_key_values.begin_step(*ids.shape)
+        return torch.zeros(3, ids.shape[1], 64)
+    monkeypatch.setattr(model.model, "forward", layers)
+    at = torch.arange(4).expand(3, 4) + 7
+    model(torch.zeros(3, 4, dtype=torch.int64), past_key_values=cache, position_ids=at)
+    model(torch.zeros(3, 1, dtype=torch.int64), past_key_values=cache)
+    assert seen[0] is at and seen[1] is None
