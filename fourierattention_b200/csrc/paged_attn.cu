@@ -510,7 +510,9 @@ static PaPlan pa_plan(const fa_paged_attn_args_t* a) {
   PaPlan pl;
   const int64_t G = a->Hq / a->Hkv;
   pl.ctas = sm_count();
-  // eight rows fill the streaming kernel's instruction; sixteen take a second one per key; more go to the tile kernel
+  // Eight rows fill the streaming kernel's instruction; sixteen take a second one per key; more go to the tile kernel.  The
+  // mean over the batch decides, since the lengths are on the device: one long prompt among many sequences of a token
+  // each is read in blocks of 16 rows.
   const int64_t own = a->cu_seqlens && a->B > 0 ? (int64_t)a->tokens * G / a->B : G, pre = (int64_t)a->tokens * G;
   pl.rows_own = a->cu_seqlens && own > 16 ? PT_ROWS : own <= 8 ? 8 : 16;
   pl.rows_pre = pre > 16 ? PT_ROWS : pre <= 8 ? 8 : 16;
@@ -521,8 +523,9 @@ static PaPlan pa_plan(const fa_paged_attn_args_t* a) {
     return r;
   };
   // Blocks that a sequence's own rows fill read the prefix no more often by themselves than packed with others', and the
-  // prefix in front of their own keys saves a launch and partial results (4 heads per group: 8 x up to 250 tokens over
-  // 16384 keys 422 us against 436 as two phases, 4 x up to 1000 over 8192 459 against 551); emptier blocks are better packed across the batch.
+  // prefix in front of their own keys saves a launch and partial results (4 heads per group, whole calls in short loops:
+  // 8 x up to 250 tokens over 16384 keys 423 us against 435 as two phases, 4 x up to 1000 over 8192 462 against 558);
+  // emptier blocks are better packed across the batch.
   pl.lead = a->prefix_len > 0 && pl.rows_own == PT_ROWS && own >= 3 * PT_ROWS / 4;
   const bool shared = a->prefix_len > 0 && !pl.lead;
   for (int i = 0; i < (shared ? 2 : 1); ++i) {

@@ -5,11 +5,13 @@
 //   O += P V    (tcgen05.mma, P from tensor memory, V as it lies in the page: the MN-major operand).
 // Bound: the tensor pipe (2 x 512 cycles per query tile and key tile at D = 128) and the exponentials (16 per cycle and
 // SM: 1024 cycles), which run side by side: the warps of one query tile work while the other's products run.  Reached is
-// 53 % of either (1.03 PFLOP/s with full blocks, 352 us for 403 GFLOP at 1.64 GHz): a query tile's chain of scores, maximum,
-// exponentials and product takes 3350 cycles per key tile.
+// 57 % of either with full blocks (8 x 256 tokens over 16384 keys, 32 / 8 heads: 554 GFLOP in 493 us at 1.64 GHz, 1.12 PFLOP/s):
+// a query tile's chain of scores, maximum, exponentials and product takes 3680 cycles per key tile, of which 2048 are the
+// products of the two query tiles.
 //   warps 0-7, 8-15  softmax of query tile 0 / 1: two threads per row, 64 keys each, which agree through one barrier with
 //                    a vote.  Four warps per scheduler cover one another's latencies better than two with 128 keys per
-//                    thread (8 x up to 250 rows of 4 heads over 16384 keys: 489 us against 517, otherwise alike).
+//                    thread (8 x up to 250 rows of 4 heads over 16384 keys, whole calls in a long loop, at
+//                    the power limit: 489 us against 517, otherwise alike).
 //   warp 16          issues the MMAs and owns tensor memory.  The issuing lane is chosen by elect.sync, descriptors are
 //                    made once: the operands then sit in uniform registers and an MMA takes ~20 cycles to issue; behind
 //                    `lane == 0`, with descriptors made per MMA, it took 100 to 160 and bound the kernel (an MMA of
@@ -30,6 +32,8 @@ namespace fa {
 
 constexpr int PT_THREADS = 640;                           // 96 registers each at launch, moved to where they are needed:
 constexpr int PT_SOFTMAX_REGS = 104, PT_OTHER_REGS = 64;   // 512 x 104 + 128 x 64 = 640 x 96
+// (the compiler reports 900 bytes of spill stores and 516 of loads at D = 128, 236 and 352 were the warps with 64 registers,
+// each with a walk over the units, given 96)
 constexpr int PT_ROWS = 256;                              // rows_log2 = 8
 
 // a stretch of one unit's tiles, as the softmax warps need it; written ahead by a warp of its own, so that the walk and

@@ -22,7 +22,7 @@
 // twice) and exchanges partial
 // results through distributed shared memory: every CTA reads all of them and decides alike, one cluster barrier per
 // step.  Bound: the latency of those steps (a cluster barrier is ~1500 cycles, a pass over the CTA's elements 4 to 12
-// thousand).  Measured: one row of 128256 27 us, 256 float32 rows 214 us (the rows' bytes alone: 20 us).  Everything is inlined:
+// thousand).  Measured: one row of 128256 27 us, 256 float32 rows 215 us (the rows' bytes alone: 20 us).  Everything is inlined:
 // with the state behind a pointer it lived in local memory, and a row took 34 us.
 #include <cooperative_groups.h>
 
@@ -851,7 +851,8 @@ struct Sampler {
 };
 
 // CTAS: how many share an SM.  Alone a CTA keeps its values in registers (118 instead of 64) and is 7 % faster; two hide
-// each other's waits (256 rows of 128256: 214 us against 306).
+// each other's waits (256 rows of 128256: 214 us against 306).  Above 131072 logits only one fits into an SM's shared memory,
+// whatever was asked for; the compiler reports 32 to 52 bytes of spills for two.
 template <typename T, int CTAS>
 __global__ void __launch_bounds__(SA_THREADS, CTAS) sample_kernel(const SampleParams p) {
   extern __shared__ float sa_xs[];

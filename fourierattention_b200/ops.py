@@ -656,7 +656,10 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens=None, p
     new token of sequence b sees ``kv_lens[b]`` keys of its own, each one before it a key less, and every token sees the
     first ``prefix_len`` keys of ``prefix_pages`` (int32 page ids).  Returns (tokens, Hq, D) of q's dtype, with
     ``return_lse`` also the log-sum-exp of the scores, (tokens, Hq) float32.  A token without any key gets 0 and
-    -infinity; tokens behind the last sequence are left as they were.  Scratch comes from PyTorch's allocator, per
+    -infinity; tokens behind the last sequence are left as they were.  Sums are float32, but each probability is rounded
+    to the pages' type before it meets its value (the tensor cores multiply equal types), so the error against exact
+    arithmetic is about a third above that of rounding the output alone: 2.3e-3 for 1.7e-3 in bfloat16, 2.5e-4 for 2.1e-4
+    in float16, relative.  A value that is not finite may make earlier new tokens of its sequence NaN.  Scratch comes from PyTorch's allocator, per
     call."""
     _no_grad(q, k_pages, v_pages)
     code, dtype = _dt(q), q.dtype

@@ -357,7 +357,9 @@ typedef struct {
 
 /* Attention of the new tokens over the prefix (all of it) and their own sequence's keys up to themselves: the last new
  * token sees kv_lens[b] keys, each one before it a key less.  The prefix is read once for the whole batch.  A row
- * without keys gives 0, lse -infinity. */
+ * without keys gives 0, lse -infinity.  Sums are float32; each probability is rounded to `dtype` before it meets its
+ * value.  A value that is not finite may make rows of earlier new tokens of its sequence NaN: theirs is a product
+ * with a probability of 0. */
 size_t fa_paged_attn_scratch_bytes(const fa_paged_attn_args_t* args_host);
 int fa_paged_attn_launches(const fa_paged_attn_args_t* args_host); /* kernels a call runs: 0 to 3 */
 int fa_paged_attn(const fa_paged_attn_args_t* args_host, fa_stream_t stream);
