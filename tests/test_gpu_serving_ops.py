@@ -847,3 +847,13 @@ def test_attention_pages_of_many_tokens(ops, ps, layout):
         own = [n + 333 * i for i, n in enumerate(new)]
         for prefix in (0, 700):
             check_attention(ops, new, own, prefix, 8, 2, 128, ps, HF, layout=layout, seed=ps, q_layout="wide", pad=1)
+
+
+@pytest.mark.parametrize("new,own,prefix,hq,hkv,d,dtype", [
+    ([2500, 1, 700], [2500, 2500, 900], 0, 8, 2, 128, BF), ([4000], [4000], 0, 4, 1, 64, HF),
+    ([512] + [1] * 255, [1500] + [100 + 3 * i for i in range(255)], 0, 8, 2, 128, BF),
+    ([512] + [1] * 255, [512] + [1 + 3 * i for i in range(255)], 333, 16, 2, 64, HF),
+    ([0] * 63 + [700], [40] * 63 + [900], 1000, 8, 2, 128, BF)])
+def test_attention_prompts_and_mixed_batches(ops, new, own, prefix, hq, hkv, d, dtype):
+    """Prompts of thousands of tokens without a prefix, one prompt among many sequences of a token each or idle ones."""
+    check_attention(ops, new, own, prefix, hq, hkv, d, 64, dtype, pad=2)
