@@ -74,7 +74,11 @@ class PagedCache(Cache):
         return self._plan
 
     def begin_step(self, rows: int, tokens: int):
-        """Makes room for the new tokens of a model call on ``(rows, tokens)`` input ids."""
+        """Makes room for the new tokens of a model call on ``(rows, tokens)`` input ids.  Host work, not to be captured: a
+        captured step is that of the layers, and this call comes before each of its replays."""
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PagedCache.begin_step cannot be captured: a replay would move on the lengths, not the pages; "
+                               "capture the layers and call begin_step before each replay")
         new = self._plan
         if new is None:
             if rows != self.batch:

@@ -285,3 +285,19 @@ def test_paged_steps_of_several_tokens_in_a_graph():
                     if n:
                         check_last(out.view(1, 8, -1)[:, :at], model, [s])
                 del other
+
+
+def test_a_step_is_not_captured_with_its_bookkeeping():
+    """A replay would lengthen the sequences on the device alone, past the pages they have."""
+    from fourierattention_b200 import PagedCache
+    model = small_model(False)
+    cache = PagedCache(2, 2, 64, 2, 64, page_size=16, dtype=torch.float16)
+    tok = torch.zeros(2, 1, dtype=torch.int64, device="cuda")
+    with torch.no_grad():
+        model(tok, past_key_values=cache)
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="captured"):
+            with torch.cuda.graph(graph):
+                model(tok, past_key_values=cache)
+        assert cache.lengths == [1, 1] and cache.kv_lens.tolist() == [1, 1]
+        assert bool(torch.isfinite(model(tok, past_key_values=cache).logits).all()) and cache.lengths == [2, 2]
