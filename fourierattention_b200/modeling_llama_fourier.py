@@ -280,7 +280,7 @@ class LlamaForCausalLM(nn.Module):
                 raise ValueError(f"num_logits_to_keep={num_logits_to_keep} of packed tokens: the rows would be of the last "
                                  "sequences only; 1 gives every sequence's last token, 0 all rows")
             mask = kwargs.get("attention_mask")
-            if mask is not None and not bool((mask != 0).all()):
+            if mask is not None and mask.dim() == 2 and not bool((mask != 0).all()):
                 raise ValueError("a PagedCache takes sequences of different lengths packed (plan), not padded behind a mask")
         positions = {}
         if isinstance(past_key_values, PagedCache) and kwargs.get("position_ids") is not None:

@@ -140,3 +140,11 @@ def test_given_positions_reach_the_layers(pkg, monkeypatch):
     model(torch.zeros(3, 4, dtype=torch.int64), past_key_values=cache, position_ids=at)
     model(torch.zeros(3, 1, dtype=torch.int64), past_key_values=cache)
     assert seen[0] is at and seen[1] is None
+
+
+def test_a_causal_mask_is_no_padding(pkg, monkeypatch):
+    """One of four dimensions, 0 where a token sees another, says what the attention does anyway."""
+    model, cache, ids = small(pkg), paged(pkg), torch.zeros(3, 4, dtype=torch.int64)
+    monkeypatch.setattr(model.model, "forward", lambda ids, past_key_values: past_key_values.begin_step(*ids.shape) or torch.zeros(3, 4, 64))
+    causal = torch.full((4, 4), float("-inf")).triu(1).expand(3, 1, 4, 4)
+    assert model(ids, past_key_values=cache, attention_mask=causal).logits.shape == (3, 1, 11)
